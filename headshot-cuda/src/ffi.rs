@@ -70,6 +70,23 @@ unsafe extern "C" {
                           d: u32, dtype: hs_dtype) -> hs_status;
     pub fn hs_attn_merge(ctx: *mut hs_ctx, x: *const c_void, out: *mut c_void, s: u32, h: u32, t: u32, d: u32,
                          dtype: hs_dtype) -> hs_status;
+    // serving: packed prompts and a paged K/V cache
+    pub fn hs_kv_append(ctx: *mut hs_ctx, q: *const c_void, k: *const c_void, v: *const c_void, q_out: *mut c_void,
+                        k_out: *mut c_void, k_cache: *mut c_void, v_cache: *mut c_void, block_table: *const c_int,
+                        kv_lens: *const c_int, cu_new: *const c_int, q_stride: u64, k_stride: u64, v_stride: u64,
+                        n_tokens: u32, n_seqs: u32, hq: u32, hkv: u32, d: u32, n_pages: u32, page_size: u32,
+                        max_pages: u32, dtype: hs_dtype, rope_sin: *const f32, rope_cos: *const f32, rope_rows: u32,
+                        prefix: u32, tokens_per_frame: u32) -> hs_status;
+    pub fn hs_attention_varlen(ctx: *mut hs_ctx, q: *const c_void, k: *const c_void, v: *const c_void,
+                               out: *mut c_void, q_stride: u64, k_stride: u64, v_stride: u64, cu_q: *const c_int,
+                               cu_k: *const c_int, total_q: u32, total_k: u32, n_seqs: u32, hq: u32, hkv: u32,
+                               d: u32, causal: c_int, dtype: hs_dtype, scale: f32) -> hs_status;
+    pub fn hs_attention_paged_workspace(ctx: *mut hs_ctx, bytes: *mut usize) -> hs_status;
+    pub fn hs_attention_paged(ctx: *mut hs_ctx, q: *const c_void, out: *mut c_void, k_cache: *const c_void,
+                              v_cache: *const c_void, block_table: *const c_int, kv_lens: *const c_int,
+                              q_stride: u64, n_seqs: u32, hq: u32, hkv: u32, d: u32, n_pages: u32, page_size: u32,
+                              max_pages: u32, dtype: hs_dtype, scale: f32, workspace: *mut c_void,
+                              workspace_bytes: usize) -> hs_status;
     // multi-GPU session (ring)
     pub fn hs_ring_shard(n: u32, world: c_int, rank: c_int, start: *mut u32, len: *mut u32) -> hs_status;
     pub fn hs_ring_plan(rank: c_int, world: c_int, step: c_int, src_block: *mut c_int, send_to: *mut c_int,

@@ -75,6 +75,10 @@ SIGNATURES = {
     "hs_rope_apply": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _i]),
     "hs_split_heads": (_i, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, _i]),
     "hs_attn_merge": (_i, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, _i]),
+    "hs_kv_append": (_i, [_vp] * 11 + [_u64] * 3 + [_u32] * 8 + [_i, _vp, _vp, _u32, _u32, _u32]),
+    "hs_attention_varlen": (_i, [_vp] * 5 + [_u64] * 3 + [_vp] * 2 + [_u32] * 6 + [_i, _i, _f32]),
+    "hs_attention_paged_workspace": (_i, [_vp, ctypes.POINTER(ctypes.c_size_t)]),
+    "hs_attention_paged": (_i, [_vp] * 7 + [_u64] + [_u32] * 7 + [_i, _f32, _vp, ctypes.c_size_t]),
     "hs_rope_periods": (_i, [_fp]),
     "hs_rope_tables": (_i, [_fp, _u32, _u32, _fp, _fp]),
 }

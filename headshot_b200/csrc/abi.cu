@@ -32,22 +32,19 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 bool valid_dtype(hs_dtype d) { return d == HS_F32 || d == HS_F16 || d == HS_BF16; }
 
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    cudaGetDevice(&prev);
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    cudaGetDevice(&cur);
-    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-  }
-};
-
 }  // namespace
 
 namespace hs {
+
+DeviceGuard::DeviceGuard(int dev) {
+  cudaGetDevice(&prev);
+  if (prev != dev) cudaSetDevice(dev);
+}
+DeviceGuard::~DeviceGuard() {
+  int cur = -1;
+  cudaGetDevice(&cur);
+  if (prev >= 0 && cur != prev) cudaSetDevice(prev);
+}
 
 hs_status abi_fail(hs_status s, const std::string& msg) { return fail(s, msg); }
 hs_status abi_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
@@ -438,6 +435,11 @@ hs_status hs_sync(hs_ctx* ctx) {
   if (status != 0) {
     cudaMemset(ctx->d_status, 0, sizeof(int));
     char buf[128];
+    if (status >= kSiteBadIndex) {
+      snprintf(buf, sizeof buf, "hs_sync: a kernel met an index outside its tensors and skipped it (site 0x%x: %s)", status,
+               bad_index_what(status));
+      return fail(HS_ERR_INVALID, buf);
+    }
     snprintf(buf, sizeof buf, "hs_sync: a kernel's bounded wait timed out (site 0x%x)", status);
     return fail(HS_ERR_TIMEOUT, buf);
   }

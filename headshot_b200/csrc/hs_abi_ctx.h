@@ -48,6 +48,13 @@ struct ProfScope {
 }  // namespace hs
 
 namespace hs {
+// Makes the context's device current for a call and restores the caller's.
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int dev);
+  ~DeviceGuard();
+};
+
 hs_status abi_fail(hs_status s, const std::string& msg);
 hs_status abi_cuda_fail(cudaError_t e, const char* what);
 cudaStream_t ctx_stream(hs_ctx* ctx);

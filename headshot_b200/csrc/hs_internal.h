@@ -169,6 +169,81 @@ cudaError_t launch_qk_prep(cudaStream_t stream, const void* x, int in_code, cons
                            int out_code, uint32_t S, uint32_t H, uint32_t t, const QkPrologue& p, int* status,
                            uint64_t timeout_ns);
 
+// ---- serving: packed prompts and the paged key-value cache --------------
+
+// Site codes from here on mean that a kernel found an index in the caller's
+// device arrays outside the tensors it indexes and skipped the access; hs_sync
+// reports them as HS_ERR_INVALID.  (Lower codes are bounded waits.)
+enum BadIndexSite : int {
+  kSiteBadIndex = 0x400,
+  kSiteBadPage = 0x401,     // block_table entry outside [0, n_pages)
+  kSiteBadLength = 0x402,   // kv_lens entry past max_pages * page_size
+  kSiteBadRopeRow = 0x403,  // position past the rotation table
+  kSiteBadOffsets = 0x404,  // cu_* not rising from 0 within the packed rows
+};
+inline const char* bad_index_what(int site) {
+  switch (site) {
+    case kSiteBadPage: return "page index";
+    case kSiteBadLength: return "cache length past the block table";
+    case kSiteBadRopeRow: return "position past the rotation table";
+    default: return "sequence offsets";
+  }
+}
+
+// A paged cache: token p of sequence s is row p % page_size of page
+// table[s * max_pages + p / page_size] in k and v (n_pages, Hkv, page_size, D).
+struct PagedCache {
+  void* k = nullptr;
+  void* v = nullptr;
+  const int* table = nullptr;
+  const int* lens = nullptr;  // tokens of each sequence
+  uint32_t n_seqs = 0, n_pages = 0, page_size = 0, max_pages = 0, heads = 0;
+};
+
+// kv_append.cu.  Rows of head vectors, `*_stride` elements from token to token.
+struct KvAppend {
+  const void* q = nullptr;  // null: no queries
+  const void* k = nullptr;
+  const void* v = nullptr;
+  void* q_out = nullptr;
+  void* k_out = nullptr;  // null: k goes to the cache only
+  uint64_t q_stride = 0, k_stride = 0, v_stride = 0;
+  const int* cu_new = nullptr;  // null: one token per sequence
+  uint32_t n_tokens = 0, q_heads = 0;
+  const float* sin_t = nullptr;  // null: no rotation
+  const float* cos_t = nullptr;
+  uint32_t rope_rows = 0, prefix = 0, tokens_per_frame = 0;
+};
+cudaError_t launch_kv_append(cudaStream_t stream, int code, uint32_t d, const KvAppend& a, const PagedCache& c,
+                             int* status);
+
+// Attention over packed sequences (token-major rows, grouped heads).
+struct VarlenIO {
+  const void* q = nullptr;
+  const void* k = nullptr;
+  const void* v = nullptr;
+  void* out = nullptr;  // (total_q, q_heads * d) contiguous
+  uint64_t q_stride = 0, k_stride = 0, v_stride = 0;
+  const int* cu_q = nullptr;
+  const int* cu_k = nullptr;
+  uint32_t total_q = 0, total_k = 0, n_seqs = 0, q_heads = 0, kv_heads = 0;
+  int causal = 0;
+};
+cudaError_t launch_attention_varlen(cudaStream_t stream, int code, uint32_t d, const VarlenIO& io, float scale,
+                                    int* status, uint64_t timeout_ns, std::string* err);
+
+// Attention of one token per sequence over the paged cache.
+struct PagedIO {
+  const void* q = nullptr;
+  void* out = nullptr;  // (n_seqs, q_heads * d) contiguous
+  uint64_t q_stride = 0;
+  uint32_t q_heads = 0;
+  void* workspace = nullptr;
+};
+size_t attention_paged_workspace_bytes();
+cudaError_t launch_attention_paged(cudaStream_t stream, int code, uint32_t d, const PagedIO& io, const PagedCache& c,
+                                   float scale, int* status);
+
 // Companion ops of the reference engine.
 cudaError_t launch_layernorm(cudaStream_t stream, const void* x, void* out, int code, const float* w,
                              const float* b, uint64_t rows, uint32_t dim, float eps);

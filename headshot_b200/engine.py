@@ -15,6 +15,13 @@ errors reported by the library raise `HsError`.
     merged = ctx.attn_merge(heads)                  # ops.rs:255-267
     out = ctx.attention_fused(q, k, v, qk_norm=QkNorm(...), rope=Rope(...))
                                                     # block.rs:136-148 as one op
+
+Serving over a growing token stream (no counterpart in the reference):
+
+    cache = PagedKv(k_pages, v_pages, block_table)
+    q = ctx.kv_append(cache, k, v, kv_lens, cu_new=cu, rope=Rope(...), q=q, k_out=k_rot)
+    out = ctx.attention_varlen(q, k_rot, v, cu)     # packed prompts, causal
+    out = ctx.attention_paged(q, cache, kv_lens)    # one new token per sequence
 """
 from __future__ import annotations
 
@@ -59,6 +66,17 @@ class Rope:
     cos: torch.Tensor
     prefix: int
     tokens_per_frame: int | None = None
+
+
+@dataclass
+class PagedKv:
+    """A paged key-value cache: k, v (n_pages, kv_heads, page_size, D) and the int32 block table
+    (n_seqs, max_pages); token p of sequence s is row p % page_size of page
+    block_table[s, p // page_size]."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    block_table: torch.Tensor
 
 
 class GpuContext:
@@ -174,6 +192,161 @@ class GpuContext:
         check(self._L.hs_attention_block_fused(
             self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(out), s, t, heads, d, _code(q),
             0.0 if scale is None else float(scale), *pro))
+        return out
+
+    # -------------------------------------------------------- serving ----
+
+    def _check_rows(self, x: torch.Tensor, name: str, heads: int | None, d: int | None) -> int:
+        """x (tokens, heads, D) with whole (heads, D) rows; returns its token stride in elements."""
+        assert x.dim() == 3, f"{name} wants (tokens, heads, D)"
+        assert heads is None or x.shape[1] == heads, f"{name} heads"
+        assert d is None or x.shape[2] == d, f"{name} head_dim"
+        assert x.is_cuda and x.device == self.device, f"{name} must live on {self.device}"
+        t, h, dd = x.shape
+        assert x.numel() == 0 or ((dd == 1 or x.stride(2) == 1) and (h == 1 or x.stride(1) == dd)), \
+            f"{name}: a token's (heads, D) must be contiguous"
+        if t <= 1 or x.numel() == 0:
+            return h * dd
+        assert x.stride(0) >= h * dd, f"{name}: tokens overlap"
+        return x.stride(0)
+
+    def _check_index(self, x: torch.Tensor, name: str, shape: tuple) -> None:
+        assert x.dtype == torch.int32, f"{name} must be int32"
+        assert tuple(x.shape) == shape, f"{name} must have shape {shape}"
+        self._check_tensor(x, name)
+
+    def _cache_args(self, cache: PagedKv, kv_lens: torch.Tensor, dtype: torch.dtype) -> tuple:
+        assert cache.k.dim() == 4 and cache.k.shape == cache.v.shape, "cache wants k, v (pages, heads, page_size, D)"
+        assert cache.k.dtype == cache.v.dtype == dtype, "cache dtype mismatch"
+        self._check_tensor(cache.k, "cache.k")
+        self._check_tensor(cache.v, "cache.v")
+        assert cache.block_table.dim() == 2, "block_table wants (n_seqs, max_pages)"
+        n_seqs = cache.block_table.shape[0]
+        self._check_index(cache.block_table, "block_table", tuple(cache.block_table.shape))
+        self._check_index(kv_lens, "kv_lens", (n_seqs,))
+        pages, _, page, _ = cache.k.shape
+        return n_seqs, pages, page, cache.block_table.shape[1]
+
+    def kv_append(self, cache: PagedKv, k: torch.Tensor, v: torch.Tensor, kv_lens: torch.Tensor,
+                  cu_new: torch.Tensor | None = None, rope: Rope | None = None, q: torch.Tensor | None = None,
+                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Writes k, v (tokens, kv_heads, D) of new tokens into the cache, k rotated by `rope`.
+
+        Sequence s owns tokens [cu_new[s], cu_new[s+1]) (one each without cu_new), its last one at
+        position kv_lens[s] - 1: kv_lens counts the tokens after the append.  Tokens whose position
+        comes out negative and tokens past cu_new[-1] are padding and left alone.  `rope` tables have
+        a row per position (tokens_per_frame None) or per frame token.  With q, returns the tokens'
+        rotated queries (q_out, allocated if not given); k_out receives the rotated keys once more,
+        as attention_varlen takes them."""
+        hkv, d = cache.k.shape[1], cache.k.shape[3]
+        n = k.shape[0]
+        assert k.dtype == v.dtype, "k/v dtype mismatch"
+        assert v.shape == k.shape, "k/v shape mismatch"
+        ks, vs = self._check_rows(k, "k", hkv, d), self._check_rows(v, "v", hkv, d)
+        n_seqs, pages, page, max_pages = self._cache_args(cache, kv_lens, k.dtype)
+        if cu_new is not None:
+            self._check_index(cu_new, "cu_new", (n_seqs + 1,))
+        else:
+            assert n == n_seqs, "without cu_new there is one token per sequence"
+        hq = qs = 0
+        if q is not None:
+            qs = self._check_rows(q, "q", None, d)
+            hq = q.shape[1]
+            assert q.shape[0] == n and q.dtype == k.dtype, "q tokens or dtype mismatch"
+            assert hq % hkv == 0, "q heads must be a multiple of k heads"
+            if q_out is None:
+                q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+            assert q_out.shape == q.shape and q_out.dtype == q.dtype, "q_out shape"
+            self._check_tensor(q_out, "q_out")
+        else:
+            assert q_out is None, "q_out without q"
+        if k_out is not None:
+            assert k_out.shape == k.shape and k_out.dtype == k.dtype, "k_out shape"
+            self._check_tensor(k_out, "k_out")
+        sin = cos = None
+        rows = prefix = tpf = 0
+        if rope is not None:
+            assert rope.sin.dtype == torch.float32 and rope.cos.dtype == torch.float32, "rope tables must be f32"
+            assert rope.sin.shape == rope.cos.shape and rope.sin.shape[-1] == d, "table size"
+            self._check_tensor(rope.sin, "rope.sin")
+            self._check_tensor(rope.cos, "rope.cos")
+            sin, cos = rope.sin, rope.cos
+            rows, prefix, tpf = rope.sin.numel() // d, rope.prefix, rope.tokens_per_frame or 0
+        if n == 0 or n_seqs == 0:
+            return q_out
+        self._bind_stream()
+        check(self._L.hs_kv_append(self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(cache.k),
+                                   _ptr(cache.v), _ptr(cache.block_table), _ptr(kv_lens), _ptr(cu_new), qs, ks, vs, n,
+                                   n_seqs, hq, hkv, d, pages, page, max_pages, _code(k), _ptr(sin), _ptr(cos), rows,
+                                   prefix, tpf))
+        return q_out
+
+    def attention_varlen(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                         cu_k: torch.Tensor | None = None, causal: bool = True, scale: float | None = None,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of packed sequences: q (tokens, heads, D), k and v (tokens, kv_heads, D); tokens
+        [cu[s], cu[s+1]) are sequence s (cu_k: other lengths for k and v).  Causal masks align to the
+        end: the last query sees every key.  Returns (tokens, heads, D); queries that see no key are
+        zero, rows past cu_q[-1] are left as they were (uninitialised where `out` is allocated here)."""
+        qs = self._check_rows(q, "q", None, None)
+        t, hq, d = q.shape
+        ks = self._check_rows(k, "k", None, d)
+        vs = self._check_rows(v, "v", None, d)
+        assert k.shape == v.shape, "k/v shape mismatch"
+        assert q.dtype == k.dtype == v.dtype, "q/k/v dtype mismatch"
+        hkv = k.shape[1]
+        assert hkv > 0 and hq % hkv == 0, "q heads must be a multiple of k heads"
+        assert cu_q.dim() == 1 and cu_q.numel() >= 1, "cu_q wants (n_seqs + 1,)"
+        n_seqs = cu_q.numel() - 1
+        self._check_index(cu_q, "cu_q", (n_seqs + 1,))
+        if cu_k is not None:
+            self._check_index(cu_k, "cu_k", (n_seqs + 1,))
+        else:
+            assert k.shape[0] == t, "without cu_k, k and v have as many tokens as q"
+        if out is None:
+            out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+        assert out.shape == q.shape and out.dtype == q.dtype, "out shape"
+        self._check_tensor(out, "out")
+        if out.numel() == 0:
+            return out
+        self._bind_stream()
+        check(self._L.hs_attention_varlen(self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(out), qs, ks, vs, _ptr(cu_q),
+                                          _ptr(cu_k), t, k.shape[0], n_seqs, hq, hkv, d, 1 if causal else 0, _code(q),
+                                          0.0 if scale is None else float(scale)))
+        return out
+
+    def paged_workspace(self) -> torch.Tensor:
+        """A workspace for attention_paged, good for every shape.  Calls that may overlap on the GPU
+        (two streams, two graphs) need one each."""
+        n = ctypes.c_size_t()
+        check(self._L.hs_attention_paged_workspace(self._h, ctypes.byref(n)))
+        return torch.zeros(n.value, dtype=torch.uint8, device=self.device)
+
+    def attention_paged(self, q: torch.Tensor, cache: PagedKv, kv_lens: torch.Tensor, scale: float | None = None,
+                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """One new token per sequence over the cache: q (n_seqs, heads, D) attends to the first
+        kv_lens[s] cached tokens; kv_lens[s] <= 0 gives zeros.  Returns (n_seqs, heads, D).  Pass a
+        paged_workspace() to spare each call the making of one."""
+        hkv, d = cache.k.shape[1], cache.k.shape[3]
+        qs = self._check_rows(q, "q", None, d)
+        n_seqs, pages, page, max_pages = self._cache_args(cache, kv_lens, q.dtype)
+        assert q.shape[0] == n_seqs, "q wants one token per sequence"
+        hq = q.shape[1]
+        assert hkv > 0 and hq % hkv == 0, "q heads must be a multiple of k heads"
+        if out is None:
+            out = torch.empty((n_seqs, hq, d), dtype=q.dtype, device=q.device)
+        assert out.shape == q.shape and out.dtype == q.dtype, "out shape"
+        self._check_tensor(out, "out")
+        if out.numel() == 0:
+            return out
+        if workspace is None:
+            workspace = self.paged_workspace()
+        self._check_tensor(workspace, "workspace")
+        self._bind_stream()
+        check(self._L.hs_attention_paged(self._h, _ptr(q), _ptr(out), _ptr(cache.k), _ptr(cache.v),
+                                         _ptr(cache.block_table), _ptr(kv_lens), qs, n_seqs, hq, hkv, d, pages, page,
+                                         max_pages, _code(q), 0.0 if scale is None else float(scale),
+                                         _ptr(workspace), workspace.numel() * workspace.element_size()))
         return out
 
     _EPILOGUES = {"none": 0, "gelu": 1, "residual_ls": 2}

@@ -106,7 +106,8 @@ HS_API hs_status hs_memset(hs_ctx* ctx, void* dst, int value, size_t bytes);
 HS_API hs_status hs_memcpy_h2d(hs_ctx* ctx, void* dst_device, const void* src_host, size_t bytes);
 HS_API hs_status hs_memcpy_d2h(hs_ctx* ctx, void* dst_host, const void* src_device, size_t bytes);
 /* Replaces GpuContext::flush + sync (src/engine/mod.rs:261-284): waits for
- * the stream and returns HS_ERR_TIMEOUT if a kernel's bounded wait fired. */
+ * the stream and returns HS_ERR_TIMEOUT if a kernel's bounded wait fired,
+ * HS_ERR_INVALID if a serving op met an index outside its tensors. */
 HS_API hs_status hs_sync(hs_ctx* ctx);
 
 /* -------------------------------------------------------------- ops ---- */
@@ -220,6 +221,80 @@ HS_API hs_status hs_split_heads(hs_ctx* ctx, const void* x, void* out, uint32_t 
 /* Replaces GpuContext::attn_merge (src/engine/ops.rs:255-267): (S, H, T, D) -> (S*T, H*D). */
 HS_API hs_status hs_attn_merge(hs_ctx* ctx, const void* x, void* out, uint32_t S, uint32_t H, uint32_t T, uint32_t D,
                         hs_dtype dtype);
+
+/* ------------------ serving: packed prompts and a paged K/V cache ------ */
+
+/* Attention over a growing stream of tokens; no counterpart in the
+ * reference (its attention is non-causal over one length,
+ * src/engine/ops.rs:225-253).  f16 and bf16 storage, D = 64 or 128, grouped
+ * heads: query head h reads key head h / (Hq / Hkv); Hq is a multiple of
+ * Hkv, both at most 1024.
+ *
+ * Layouts.  Tokens are packed without padding, head vectors side by side:
+ * row t of q is (Hq, D) at q + t * q_stride elements (k and v with Hkv), so a
+ * fused projection's output is read in place; a stride of 0 means Hq*D
+ * (Hkv*D), others are multiples of 8 that cover the heads.  The cache is
+ * k_cache, v_cache (n_pages, Hkv, page_size, D), any page_size >= 1; token p
+ * of sequence s is row p % page_size of page
+ * block_table[s * max_pages + p / page_size].  Pointers to vectors and
+ * tables are 16-byte aligned.
+ *
+ * Index arrays (block_table, kv_lens, cu_*) are device ints, read when the
+ * kernel runs, so a captured graph follows their current values.  kv_lens[s]
+ * is the length of sequence s with the tokens of the running step.  An index
+ * that points outside its tensors is skipped, never followed: hs_sync then
+ * returns HS_ERR_INVALID and names it. */
+
+/* Appends n_tokens new keys and values to the cache.  cu_new (n_seqs + 1,
+ * rising from 0): sequence s owns tokens [cu_new[s], cu_new[s+1]), the last
+ * of which takes position kv_lens[s] - 1; NULL: one token per sequence
+ * (n_tokens == n_seqs).  A token whose position comes out negative, and
+ * tokens from cu_new[n_seqs] on, are padding: nothing of them is read or
+ * written.  Two tokens of one call must not share a cache row.
+ * rope_sin != NULL rotates k, and q if given, as hs_rope_apply does: table
+ * row of position p is (p mod tokens_per_frame) - prefix, p itself for
+ * tokens_per_frame == 0; rows below 0 pass through.  Tables (rope_rows, D).
+ * q (may be NULL, then q_out is NULL): the tokens' queries, rotated into
+ * q_out (n_tokens, Hq, D).  k_out (may be NULL): the rotated keys once more,
+ * (n_tokens, Hkv, D), for hs_attention_varlen.  q_out may be q and k_out may
+ * be k where those are contiguous. */
+HS_API hs_status hs_kv_append(hs_ctx* ctx, const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                              void* k_cache, void* v_cache, const int* block_table, const int* kv_lens,
+                              const int* cu_new, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
+                              uint32_t n_tokens, uint32_t n_seqs, uint32_t Hq, uint32_t Hkv, uint32_t D,
+                              uint32_t n_pages, uint32_t page_size, uint32_t max_pages, hs_dtype dtype,
+                              const float* rope_sin, const float* rope_cos, uint32_t rope_rows, uint32_t prefix,
+                              uint32_t tokens_per_frame);
+
+/* Attention of packed sequences: tokens [cu_q[s], cu_q[s+1]) of q attend to
+ * tokens [cu_k[s], cu_k[s+1]) of k and v (cu_k NULL: cu_q, total_k ==
+ * total_q).  causal: query i of Lq sees keys j <= i + Lk - Lq (the last query
+ * sees every key); else all Lk.  A query that sees none is zero.  out
+ * (total_q, Hq*D); rows from cu_q[n_seqs] on are left as they were.  Keys
+ * and values past a sequence's end never take part, whatever they hold; the
+ * values of a sequence's own keys must be finite.  Hq / Hkv <= 128.
+ * scale <= 0 selects 1/sqrt(D). */
+HS_API hs_status hs_attention_varlen(hs_ctx* ctx, const void* q, const void* k, const void* v, void* out,
+                                     uint64_t q_stride, uint64_t k_stride, uint64_t v_stride, const int* cu_q,
+                                     const int* cu_k, uint32_t total_q, uint32_t total_k, uint32_t n_seqs,
+                                     uint32_t Hq, uint32_t Hkv, uint32_t D, int causal, hs_dtype dtype, float scale);
+
+/* Bytes of the workspace hs_attention_paged needs on this device: one size
+ * for every shape.  Zero it once (hs_memset); each call leaves it ready for
+ * the next.  Calls that may overlap on the GPU (two streams, two graphs)
+ * need one each. */
+HS_API hs_status hs_attention_paged_workspace(hs_ctx* ctx, size_t* bytes);
+
+/* One new token per sequence against its cache: q (n_seqs, Hq, D) at
+ * q_stride attends to the first kv_lens[s] cached tokens; out (n_seqs,
+ * Hq*D).  kv_lens[s] <= 0 gives a zero row.  The cache's length is split over
+ * the GPU and joined within the call, in an order that depends on the
+ * lengths only, so equal calls give equal bits.  scale as above. */
+HS_API hs_status hs_attention_paged(hs_ctx* ctx, const void* q, void* out, const void* k_cache, const void* v_cache,
+                                    const int* block_table, const int* kv_lens, uint64_t q_stride, uint32_t n_seqs,
+                                    uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size,
+                                    uint32_t max_pages, hs_dtype dtype, float scale, void* workspace,
+                                    size_t workspace_bytes);
 
 /* --------------------------------------- multi-GPU session (ring) ------ */
 

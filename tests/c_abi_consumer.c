@@ -49,6 +49,8 @@ static const any_fn entry_points[] = {
     FN(hs_ring_ulysses_attention_fused),
     FN(hs_copy_row_blocks),
     FN(hs_im2col_patch),          FN(hs_cache_build),
+    FN(hs_kv_append),             FN(hs_attention_varlen),
+    FN(hs_attention_paged),       FN(hs_attention_paged_workspace),
     FN(hs_rope_periods),          FN(hs_rope_tables),
 };
 
