@@ -1,5 +1,4 @@
-// attention_serving.cu — attention over packed sequences and over a paged
-// cache, one warp per (query token, query head).
+// attention_serving.cu — attention over packed sequences, one warp per (query token, query head).
 //
 // out = sum_j p_j v_j / sum_j p_j with p_j = 2^(s_j c - m), s_j = q.k_j and
 // c = scale log2 e, over the keys the mask leaves; m is the running maximum,
@@ -95,32 +94,6 @@ __global__ void __launch_bounds__(32 * kWarps) varlen_kernel(const VarlenIO io, 
   }
 }
 
-template <typename E, int D>
-__global__ void __launch_bounds__(32 * kWarps) paged_kernel(const PagedIO io, const PagedCache c, float scale_log2,
-                                                            int* status) {
-  const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const uint32_t seq = static_cast<uint32_t>(row / io.q_heads), head = static_cast<uint32_t>(row % io.q_heads);
-  if (seq >= c.n_seqs) return;
-  int64_t keys = c.lens[seq];
-  const int64_t room = static_cast<int64_t>(c.max_pages) * c.page_size;
-  if (keys > room) {
-    atomicCAS(status, 0, static_cast<int>(kSiteBadLength));
-    keys = room;
-  }
-  const uint32_t kv = head / (io.q_heads / c.heads);
-  attend<E, D>(static_cast<const E*>(io.q) + seq * io.q_stride + head * D, static_cast<E*>(io.out) + row * D, keys,
-               scale_log2, [&](int64_t j, const E** k, const E** v) {
-                 const int page = c.table[static_cast<uint64_t>(seq) * c.max_pages + j / c.page_size];
-                 if (page < 0 || static_cast<uint32_t>(page) >= c.n_pages) {
-                   atomicCAS(status, 0, static_cast<int>(kSiteBadPage));
-                   return;
-                 }
-                 const uint64_t at = ((static_cast<uint64_t>(page) * c.heads + kv) * c.page_size + j % c.page_size) * D;
-                 *k = static_cast<const E*>(c.k) + at;
-                 *v = static_cast<const E*>(c.v) + at;
-               });
-}
-
 }  // namespace
 
 cudaError_t launch_attention_varlen(cudaStream_t stream, int code, uint32_t d, const VarlenIO& io, float scale,
@@ -136,20 +109,6 @@ cudaError_t launch_attention_varlen(cudaStream_t stream, int code, uint32_t d, c
   else if (code == kBF16) varlen_kernel<__nv_bfloat16, 128><<<g, b, 0, stream>>>(io, c, status);
   else if (d == 64) varlen_kernel<__half, 64><<<g, b, 0, stream>>>(io, c, status);
   else varlen_kernel<__half, 128><<<g, b, 0, stream>>>(io, c, status);
-  return cudaGetLastError();
-}
-
-size_t attention_paged_workspace_bytes() { return 256; }
-
-cudaError_t launch_attention_paged(cudaStream_t stream, int code, uint32_t d, const PagedIO& io, const PagedCache& c,
-                                   float scale, int* status) {
-  const uint64_t blocks = (static_cast<uint64_t>(c.n_seqs) * io.q_heads + kWarps - 1) / kWarps;
-  const float s = scale * 1.4426950408889634f;
-  const dim3 g(static_cast<uint32_t>(blocks)), b(32 * kWarps);
-  if (code == kBF16 && d == 64) paged_kernel<__nv_bfloat16, 64><<<g, b, 0, stream>>>(io, c, s, status);
-  else if (code == kBF16) paged_kernel<__nv_bfloat16, 128><<<g, b, 0, stream>>>(io, c, s, status);
-  else if (d == 64) paged_kernel<__half, 64><<<g, b, 0, stream>>>(io, c, s, status);
-  else paged_kernel<__half, 128><<<g, b, 0, stream>>>(io, c, s, status);
   return cudaGetLastError();
 }
 
