@@ -8,9 +8,10 @@
 // it; a single short sequence is bound by latency.
 //
 // Work is cut in tiles of 64 keys of one (sequence, key head, head tile)
-// item, numbered through all items.  The grid is fixed; each CTA finds the
+// item, numbered through all items (an item has kItemCost numbers more than
+// tiles, for its end).  The grid is fixed; each CTA finds the
 // total from the lengths on the device and takes an equal contiguous range of
-// tiles, so ragged batches and single long sequences load every SM alike and
+// numbers, so ragged batches and single long sequences load every SM alike and
 // the host needs no lengths (a captured graph follows them).  An item that
 // one CTA covers is written directly.  One that is cut leaves a partial
 // (m, l, O) per CTA in the workspace; the last CTA to arrive at the item's
@@ -57,7 +58,14 @@ struct Shape {
   static constexpr int kSmem = kWarps * kStages * kStageBytes;
 };
 
-constexpr uint32_t kMinTiles = 4;  // per CTA: below 256 keys the join costs more than the keys
+// An item's end costs a CTA about as much as two tiles (query loads, the join
+// of the warps), so each item takes two numbers more than its tiles: 128
+// sequences of 1 to 16,001 keys, 219 us without them, 165 us with 1, 2 or 4.
+constexpr uint32_t kItemCost = 2;
+// Fewest numbers per CTA: with 2, 64 sequences of 100 keys (two tiles an
+// item) take 13.6 us instead of 12.6, because items that fit one CTA are cut;
+// with 8, 17.0 us.
+constexpr uint32_t kMinTiles = 4;
 
 // Workspace: counters, then per CTA two partials of (16 x 128 O, 16 m, 16 l) f32.
 constexpr size_t kCounterBytes = kMaxCtas * sizeof(uint32_t);
@@ -123,11 +131,14 @@ __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return len ? (len +
 
 // A place in the numbering of tiles: tile `tile` of item (seq, sub).
 struct Place {
+  unsigned long long at;  // in the numbering
   uint32_t seq, sub, tile, tiles, len;
 };
 
 __device__ __forceinline__ void next_tile(const Args& a, Place& p) {
+  ++p.at;
   if (++p.tile < p.tiles) return;
+  p.at += kItemCost;
   p.tile = 0;
   if (++p.sub < a.subs) return;
   p.sub = 0;
@@ -146,7 +157,7 @@ struct Shared {
   float l[kWarps][kRows];
 };
 
-// Sum over the block, and (when asked) the exclusive prefix of this thread.
+// Sum over the block, and the exclusive prefix of this thread.
 __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, Shared* sh, unsigned long long* excl) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long inc = v;
@@ -164,7 +175,7 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, S
     if (w < warp) before += sh->sum[w];
     total += sh->sum[w];
   }
-  if (excl) *excl = before + inc - v;
+  *excl = before + inc - v;
   return total;
 }
 
@@ -223,50 +234,62 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
   __shared__ Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  // The CTA's range of tiles.
-  unsigned long long sum = 0;
-  for (uint32_t s = tid; s < a.c.n_seqs; s += kThreads) sum += tiles_of(seq_len(a, s));
-  const unsigned long long total = block_scan(sum, &sh, nullptr) * a.subs;
+  // The CTA's range of numbers, and the sequence it starts in.  `first` and
+  // `n` are this thread's sequence of the chunk scanned last.
+  auto numbers = [&](uint32_t s) -> uint32_t { return s < a.c.n_seqs ? tiles_of(seq_len(a, s)) + kItemCost : 0u; };
+  uint32_t n = numbers(tid);
+  unsigned long long first;
+  unsigned long long chunk = block_scan(n, &sh, &first);
+  unsigned long long total = chunk;
+  if (a.c.n_seqs > kThreads) {
+    unsigned long long rest = 0;
+    for (uint32_t s = tid + kThreads; s < a.c.n_seqs; s += kThreads) rest += numbers(s);
+    unsigned long long unused;
+    total += block_scan(rest, &sh, &unused);
+  }
+  total *= a.subs;
   const unsigned long long even = (total + gridDim.x - 1) / gridDim.x;
   const unsigned long long per = even < kMinTiles ? kMinTiles : even;
   const unsigned long long start = blockIdx.x * per;
   if (start >= total) return;
   const unsigned long long end = start + per < total ? start + per : total;
   unsigned long long base = 0;
-  for (uint32_t s0 = 0; s0 < a.c.n_seqs; s0 += kThreads) {
-    const uint32_t s = s0 + tid;
-    const uint32_t n = s < a.c.n_seqs ? tiles_of(seq_len(a, s)) : 0;
-    unsigned long long excl;
-    const unsigned long long chunk = block_scan(n, &sh, &excl);
-    if ((base + chunk) * a.subs > start) {
-      const unsigned long long first = (base + excl) * a.subs;
-      if (first <= start && start < first + static_cast<unsigned long long>(n) * a.subs) {
-        sh.start_seq = s;
-        sh.start_off = start - first;
-      }
-      break;
-    }
+  uint32_t s0 = 0;
+  while ((base + chunk) * a.subs <= start) {
     base += chunk;
+    s0 += kThreads;
+    if (s0 >= a.c.n_seqs) return;
+    n = numbers(s0 + tid);
+    chunk = block_scan(n, &sh, &first);
+  }
+  first = (base + first) * a.subs;
+  if (first <= start && start < first + static_cast<unsigned long long>(n) * a.subs) {
+    sh.start_seq = s0 + tid;
+    sh.start_off = start - first;
   }
   __syncthreads();
   Place cur;
   cur.seq = sh.start_seq;
   cur.len = seq_len(a, cur.seq);
   cur.tiles = tiles_of(cur.len);
-  cur.sub = static_cast<uint32_t>(sh.start_off / cur.tiles);
-  cur.tile = static_cast<uint32_t>(sh.start_off % cur.tiles);
+  cur.sub = static_cast<uint32_t>(sh.start_off / (cur.tiles + kItemCost));
+  cur.tile = static_cast<uint32_t>(sh.start_off % (cur.tiles + kItemCost));
+  cur.at = start;
+  if (cur.tile >= cur.tiles) {  // starts among an item's extra numbers: on to the next item
+    cur.at -= cur.tile - (cur.tiles - 1);
+    cur.tile = cur.tiles - 1;
+    next_tile(a, cur);
+  }
 
   const uint32_t my_ring = smem_u32(ring) + warp * S::kStages * S::kStageBytes;
-  const unsigned long long n_tiles = end - start;
   Place ahead = cur;
-  unsigned long long loaded = 0;
+  uint32_t load_stage = 0;
   auto load_next = [&] {
-    if (loaded < n_tiles) {
-      load_tile<E, D, kWholeSteps>(a, ahead, my_ring + static_cast<uint32_t>(loaded % S::kStages) * S::kStageBytes,
-                                   warp, lane);
+    if (ahead.at < end) {
+      load_tile<E, D, kWholeSteps>(a, ahead, my_ring + load_stage * S::kStageBytes, warp, lane);
       next_tile(a, ahead);
     }
-    ++loaded;
+    load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
     cp_async_commit();
   };
 #pragma unroll
@@ -278,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
   const uint32_t row_lo = lane >> 2;  // rows row_lo and row_lo + 8 of the head tile
 
   bool fresh = true;                  // the next tile starts a segment
-  for (unsigned long long i = 0; i < n_tiles; ++i) {
+  for (uint32_t st = 0; cur.at < end; st = st + 1 == S::kStages ? 0 : st + 1) {
     const uint32_t head = cur.sub / a.head_tiles;
     const uint32_t row0 = (cur.sub % a.head_tiles) * kRows;
     const uint32_t rows = min(static_cast<uint32_t>(kRows), a.group - row0);
@@ -303,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
     cp_async_wait<S::kStages - 2>();
     __syncwarp();
     load_next();
-    const uint32_t stage = my_ring + static_cast<uint32_t>(i % S::kStages) * S::kStageBytes;
+    const uint32_t stage = my_ring + st * S::kStageBytes;
     const uint32_t key0 = cur.tile * kTileKeys + warp * kWarpKeys;
     if (key0 < cur.len) {
       // Scores: rows = heads, two 8-key column tiles.
@@ -352,11 +375,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float base_m = m[h] == -INFINITY ? 0.f : m[h];
-          const uint32_t w = Elem<E>::pack2(ex2_approx(fmaf(s[t][2 * h], a.scale_log2, -base_m)),
-                                            ex2_approx(fmaf(s[t][2 * h + 1], a.scale_log2, -base_m)));
+          const float e0 = ex2_approx(fmaf(s[t][2 * h], a.scale_log2, -base_m));
+          const float e1 = ex2_approx(fmaf(s[t][2 * h + 1], a.scale_log2, -base_m));
+          const uint32_t w = Elem<E>::pack2(e0, e1);
+          p[2 * t + h] = w;
           const float2 f = Elem<E>::unpack2(w);
           l[h] += f.x + f.y;
-          p[2 * t + h] = w;
         }
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {
@@ -369,12 +393,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
     }
 
     const bool item_ends = cur.tile + 1 == cur.tiles;
-    if (item_ends || i + 1 == n_tiles) {
+    if (item_ends || cur.at + 1 == end) {
       // Join the warps: states through the stage this tile came from (its next
       // load is issued one iteration on, behind the block barrier below).
       __syncwarp();
-      float* dump = reinterpret_cast<float*>(ring + warp * S::kStages * S::kStageBytes +
-                                             static_cast<uint32_t>(i % S::kStages) * S::kStageBytes);
+      float* dump = reinterpret_cast<float*>(ring + (warp * S::kStages + st) * S::kStageBytes);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t r = row_lo + 8 * h;
@@ -393,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
         }
       }
       __syncthreads();
-      const unsigned long long item0 = start + i - cur.tile;  // first tile of the item
+      const unsigned long long item0 = cur.at - cur.tile;  // first tile of the item
       const unsigned long long item1 = item0 + cur.tiles;
       const uint32_t cta0 = static_cast<uint32_t>(item0 / per), cta1 = static_cast<uint32_t>((item1 - 1) / per);
       const bool whole = cta0 == cta1;
@@ -415,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
           const float f = sh.m[w][r] == -INFINITY ? 0.f : ex2_approx(sh.m[w][r] - mt);
           lt = fmaf(sh.l[w][r], f, lt);
           const float4 v = *reinterpret_cast<const float4*>(
-              ring + (w * S::kStages + static_cast<uint32_t>(i % S::kStages)) * S::kStageBytes +
+              ring + (w * S::kStages + st) * S::kStageBytes +
               (r * D + (c4 ^ ((r & 3) << 3))) * 4);
           acc.x = fmaf(v.x, f, acc.x);
           acc.y = fmaf(v.y, f, acc.y);
@@ -443,20 +466,40 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
           __threadfence();
           for (uint32_t e = tid; e < rows * (D / 4); e += kThreads) {
             const uint32_t r = e / (D / 4), c4 = (e % (D / 4)) * 4;
+            // In batches whose loads are all in flight together.
+            constexpr uint32_t kPart = 16;
             float mt = -INFINITY, lt = 0.f;
-            for (uint32_t c = cta0; c <= cta1; ++c) mt = fmaxf(mt, __ldcg(partial(c) + kRows * D + r));
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (uint32_t c = cta0; c <= cta1; ++c) {
-              const float* src = partial(c);
-              const float mc = __ldcg(src + kRows * D + r);
-              const float f = mc == -INFINITY ? 0.f : ex2_approx(mc - mt);
-              lt = fmaf(__ldcg(src + kRows * D + kRows + r), f, lt);
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(src + r * D + c4));
-              acc.x = fmaf(v.x, f, acc.x);
-              acc.y = fmaf(v.y, f, acc.y);
-              acc.z = fmaf(v.z, f, acc.z);
-              acc.w = fmaf(v.w, f, acc.w);
+            for (uint32_t c0 = cta0; c0 <= cta1; c0 += kPart) {
+              float mc[kPart], lc[kPart];
+              float4 v[kPart];
+#pragma unroll
+              for (uint32_t x = 0; x < kPart; ++x) {
+                const bool have = c0 + x <= cta1;
+                const float* src = partial(c0 + x);
+                mc[x] = have ? __ldcg(src + kRows * D + r) : -INFINITY;
+                lc[x] = have ? __ldcg(src + kRows * D + kRows + r) : 0.f;
+                v[x] = have ? __ldcg(reinterpret_cast<const float4*>(src + r * D + c4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              }
+              float m_new = mt;
+#pragma unroll
+              for (uint32_t x = 0; x < kPart; ++x) m_new = fmaxf(m_new, mc[x]);
+              const float f0 = mt == -INFINITY ? 0.f : ex2_approx(mt - m_new);
+              mt = m_new;
+              lt *= f0;
+              acc.x *= f0;
+              acc.y *= f0;
+              acc.z *= f0;
+              acc.w *= f0;
+#pragma unroll
+              for (uint32_t x = 0; x < kPart; ++x) {
+                const float f = mc[x] == -INFINITY ? 0.f : ex2_approx(mc[x] - mt);
+                lt = fmaf(lc[x], f, lt);
+                acc.x = fmaf(v[x].x, f, acc.x);
+                acc.y = fmaf(v[x].y, f, acc.y);
+                acc.z = fmaf(v[x].z, f, acc.z);
+                acc.w = fmaf(v[x].w, f, acc.w);
+              }
             }
             const float inv = lt == 0.f ? 0.f : 1.f / lt;
             *reinterpret_cast<uint2*>(out + r * D + c4) =

@@ -41,8 +41,8 @@ def _code(t: torch.Tensor) -> int:
     return _DTYPES[t.dtype]
 
 
-def _ptr(t: torch.Tensor | None):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 @dataclass
@@ -88,6 +88,7 @@ class GpuContext:
         check(self._L.hs_ctx_create(device, ctypes.byref(h)))
         self._h = h
         self.device = torch.device("cuda", device)
+        self._index = device  # what get_device() of a tensor on it returns
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -106,10 +107,10 @@ class GpuContext:
 
     def _bind_stream(self) -> None:
         # Order our launches with torch's work on the same device.
-        check(self._L.hs_ctx_set_stream(self._h, ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)))
+        check(self._L.hs_ctx_set_stream(self._h, torch._C._cuda_getCurrentRawStream(self._index)))
 
     def _check_tensor(self, t: torch.Tensor, name: str) -> None:
-        assert t.is_cuda and t.device == self.device, f"{name} must live on {self.device}"
+        assert t.get_device() == self._index, f"{name} must live on {self.device}"
         assert t.is_contiguous(), f"{name} must be contiguous"
 
     # ------------------------------------------------------------ ops ----
@@ -196,36 +197,41 @@ class GpuContext:
 
     # -------------------------------------------------------- serving ----
 
-    def _check_rows(self, x: torch.Tensor, name: str, heads: int | None, d: int | None) -> int:
-        """x (tokens, heads, D) with whole (heads, D) rows; returns its token stride in elements."""
+    def _check_rows(self, x: torch.Tensor, name: str) -> tuple[int, int, int, int]:
+        """x (tokens, heads, D) with whole (heads, D) rows: its sizes and its token stride in elements."""
         assert x.dim() == 3, f"{name} wants (tokens, heads, D)"
-        assert heads is None or x.shape[1] == heads, f"{name} heads"
-        assert d is None or x.shape[2] == d, f"{name} head_dim"
-        assert x.is_cuda and x.device == self.device, f"{name} must live on {self.device}"
-        t, h, dd = x.shape
-        assert x.numel() == 0 or ((dd == 1 or x.stride(2) == 1) and (h == 1 or x.stride(1) == dd)), \
-            f"{name}: a token's (heads, D) must be contiguous"
-        if t <= 1 or x.numel() == 0:
-            return h * dd
-        assert x.stride(0) >= h * dd, f"{name}: tokens overlap"
-        return x.stride(0)
+        assert x.get_device() == self._index, f"{name} must live on {self.device}"
+        t, h, d = x.shape
+        if x.is_contiguous():
+            return t, h, d, h * d
+        st, sh, sd = x.stride()
+        assert (d == 1 or sd == 1) and (h == 1 or sh == d), f"{name}: a token's (heads, D) must be contiguous"
+        if t == 1:
+            return t, h, d, h * d
+        assert st >= h * d, f"{name}: tokens overlap"
+        return t, h, d, st
 
     def _check_index(self, x: torch.Tensor, name: str, shape: tuple) -> None:
-        assert x.dtype == torch.int32, f"{name} must be int32"
-        assert tuple(x.shape) == shape, f"{name} must have shape {shape}"
+        assert x.dtype is torch.int32, f"{name} must be int32"
+        assert x.shape == shape, f"{name} must have shape {shape}"
         self._check_tensor(x, name)
 
-    def _cache_args(self, cache: PagedKv, kv_lens: torch.Tensor, dtype: torch.dtype) -> tuple:
-        assert cache.k.dim() == 4 and cache.k.shape == cache.v.shape, "cache wants k, v (pages, heads, page_size, D)"
-        assert cache.k.dtype == cache.v.dtype == dtype, "cache dtype mismatch"
-        self._check_tensor(cache.k, "cache.k")
-        self._check_tensor(cache.v, "cache.v")
-        assert cache.block_table.dim() == 2, "block_table wants (n_seqs, max_pages)"
-        n_seqs = cache.block_table.shape[0]
-        self._check_index(cache.block_table, "block_table", tuple(cache.block_table.shape))
+    def _check_cache(self, cache: PagedKv, kv_lens: torch.Tensor, dtype: torch.dtype) -> tuple:
+        """(n_seqs, max_pages, pages, kv_heads, page_size, D)."""
+        k, v, table = cache.k, cache.v, cache.block_table
+        assert k.dim() == 4 and k.shape == v.shape, "cache wants k, v (pages, heads, page_size, D)"
+        assert k.dtype is dtype and v.dtype is dtype, "cache dtype mismatch"
+        assert table.dim() == 2, "block_table wants (n_seqs, max_pages)"
+        n_seqs, max_pages = table.shape
+        self._check_tensor(k, "cache.k")
+        self._check_tensor(v, "cache.v")
+        self._check_index(table, "block_table", (n_seqs, max_pages))
         self._check_index(kv_lens, "kv_lens", (n_seqs,))
-        pages, _, page, _ = cache.k.shape
-        return n_seqs, pages, page, cache.block_table.shape[1]
+        return n_seqs, max_pages, *k.shape
+
+    def _check_out(self, out: torch.Tensor, like: torch.Tensor, name: str) -> None:
+        assert out.shape == like.shape and out.dtype is like.dtype, f"{name} shape"
+        self._check_tensor(out, name)
 
     def kv_append(self, cache: PagedKv, k: torch.Tensor, v: torch.Tensor, kv_lens: torch.Tensor,
                   cu_new: torch.Tensor | None = None, rope: Rope | None = None, q: torch.Tensor | None = None,
@@ -238,47 +244,46 @@ class GpuContext:
         a row per position (tokens_per_frame None) or per frame token.  With q, returns the tokens'
         rotated queries (q_out, allocated if not given); k_out receives the rotated keys once more,
         as attention_varlen takes them."""
-        hkv, d = cache.k.shape[1], cache.k.shape[3]
-        n = k.shape[0]
-        assert k.dtype == v.dtype, "k/v dtype mismatch"
-        assert v.shape == k.shape, "k/v shape mismatch"
-        ks, vs = self._check_rows(k, "k", hkv, d), self._check_rows(v, "v", hkv, d)
-        n_seqs, pages, page, max_pages = self._cache_args(cache, kv_lens, k.dtype)
+        dtype = k.dtype
+        n, hkv, d, ks = self._check_rows(k, "k")
+        nv, hv, dv, vs = self._check_rows(v, "v")
+        assert v.dtype is dtype, "k/v dtype mismatch"
+        assert nv == n and hv == hkv and dv == d, "k/v shape mismatch"
+        n_seqs, max_pages, pages, ch, page, cd = self._check_cache(cache, kv_lens, dtype)
+        assert ch == hkv and cd == d, "cache wants the heads and head_dim of k"
         if cu_new is not None:
             self._check_index(cu_new, "cu_new", (n_seqs + 1,))
         else:
             assert n == n_seqs, "without cu_new there is one token per sequence"
         hq = qs = 0
         if q is not None:
-            qs = self._check_rows(q, "q", None, d)
-            hq = q.shape[1]
-            assert q.shape[0] == n and q.dtype == k.dtype, "q tokens or dtype mismatch"
+            nq, hq, dq, qs = self._check_rows(q, "q")
+            assert nq == n and dq == d and q.dtype is dtype, "q tokens, head_dim or dtype mismatch"
             assert hq % hkv == 0, "q heads must be a multiple of k heads"
             if q_out is None:
-                q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
-            assert q_out.shape == q.shape and q_out.dtype == q.dtype, "q_out shape"
-            self._check_tensor(q_out, "q_out")
+                q_out = torch.empty((n, hq, d), dtype=dtype, device=q.device)
+            else:
+                self._check_out(q_out, q, "q_out")
         else:
             assert q_out is None, "q_out without q"
         if k_out is not None:
-            assert k_out.shape == k.shape and k_out.dtype == k.dtype, "k_out shape"
-            self._check_tensor(k_out, "k_out")
+            self._check_out(k_out, k, "k_out")
         sin = cos = None
         rows = prefix = tpf = 0
         if rope is not None:
-            assert rope.sin.dtype == torch.float32 and rope.cos.dtype == torch.float32, "rope tables must be f32"
-            assert rope.sin.shape == rope.cos.shape and rope.sin.shape[-1] == d, "table size"
-            self._check_tensor(rope.sin, "rope.sin")
-            self._check_tensor(rope.cos, "rope.cos")
             sin, cos = rope.sin, rope.cos
-            rows, prefix, tpf = rope.sin.numel() // d, rope.prefix, rope.tokens_per_frame or 0
+            assert sin.dtype is torch.float32 and cos.dtype is torch.float32, "rope tables must be f32"
+            assert sin.shape == cos.shape and sin.shape[-1] == d, "table size"
+            self._check_tensor(sin, "rope.sin")
+            self._check_tensor(cos, "rope.cos")
+            rows, prefix, tpf = sin.numel() // d, rope.prefix, rope.tokens_per_frame or 0
         if n == 0 or n_seqs == 0:
             return q_out
         self._bind_stream()
-        check(self._L.hs_kv_append(self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(cache.k),
-                                   _ptr(cache.v), _ptr(cache.block_table), _ptr(kv_lens), _ptr(cu_new), qs, ks, vs, n,
-                                   n_seqs, hq, hkv, d, pages, page, max_pages, _code(k), _ptr(sin), _ptr(cos), rows,
-                                   prefix, tpf))
+        check(self._L.hs_kv_append(self._h, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), _ptr(k_out),
+                                   cache.k.data_ptr(), cache.v.data_ptr(), cache.block_table.data_ptr(),
+                                   kv_lens.data_ptr(), _ptr(cu_new), qs, ks, vs, n, n_seqs, hq, hkv, d, pages, page,
+                                   max_pages, _code(k), _ptr(sin), _ptr(cos), rows, prefix, tpf))
         return q_out
 
     def attention_varlen(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -288,13 +293,11 @@ class GpuContext:
         [cu[s], cu[s+1]) are sequence s (cu_k: other lengths for k and v).  Causal masks align to the
         end: the last query sees every key.  Returns (tokens, heads, D); queries that see no key are
         zero, rows past cu_q[-1] are left as they were (uninitialised where `out` is allocated here)."""
-        qs = self._check_rows(q, "q", None, None)
-        t, hq, d = q.shape
-        ks = self._check_rows(k, "k", None, d)
-        vs = self._check_rows(v, "v", None, d)
-        assert k.shape == v.shape, "k/v shape mismatch"
-        assert q.dtype == k.dtype == v.dtype, "q/k/v dtype mismatch"
-        hkv = k.shape[1]
+        t, hq, d, qs = self._check_rows(q, "q")
+        tk, hkv, dk, ks = self._check_rows(k, "k")
+        tv, hv, dv, vs = self._check_rows(v, "v")
+        assert tk == tv and hkv == hv and dk == d and dv == d, "q/k/v shape mismatch"
+        assert q.dtype is k.dtype and q.dtype is v.dtype, "q/k/v dtype mismatch"
         assert hkv > 0 and hq % hkv == 0, "q heads must be a multiple of k heads"
         assert cu_q.dim() == 1 and cu_q.numel() >= 1, "cu_q wants (n_seqs + 1,)"
         n_seqs = cu_q.numel() - 1
@@ -302,17 +305,17 @@ class GpuContext:
         if cu_k is not None:
             self._check_index(cu_k, "cu_k", (n_seqs + 1,))
         else:
-            assert k.shape[0] == t, "without cu_k, k and v have as many tokens as q"
+            assert tk == t, "without cu_k, k and v have as many tokens as q"
         if out is None:
             out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
-        assert out.shape == q.shape and out.dtype == q.dtype, "out shape"
-        self._check_tensor(out, "out")
+        else:
+            self._check_out(out, q, "out")
         if out.numel() == 0:
             return out
         self._bind_stream()
-        check(self._L.hs_attention_varlen(self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(out), qs, ks, vs, _ptr(cu_q),
-                                          _ptr(cu_k), t, k.shape[0], n_seqs, hq, hkv, d, 1 if causal else 0, _code(q),
-                                          0.0 if scale is None else float(scale)))
+        check(self._L.hs_attention_varlen(self._h, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs, ks, vs,
+                                          cu_q.data_ptr(), _ptr(cu_k), t, tk, n_seqs, hq, hkv, d, 1 if causal else 0,
+                                          _code(q), 0.0 if scale is None else scale))
         return out
 
     def paged_workspace(self) -> torch.Tensor:
@@ -327,26 +330,26 @@ class GpuContext:
         """One new token per sequence over the cache: q (n_seqs, heads, D) attends to the first
         kv_lens[s] cached tokens; kv_lens[s] <= 0 gives zeros.  Returns (n_seqs, heads, D).  Pass a
         paged_workspace() to spare each call the making of one."""
-        hkv, d = cache.k.shape[1], cache.k.shape[3]
-        qs = self._check_rows(q, "q", None, d)
-        n_seqs, pages, page, max_pages = self._cache_args(cache, kv_lens, q.dtype)
-        assert q.shape[0] == n_seqs, "q wants one token per sequence"
-        hq = q.shape[1]
+        n, hq, d, qs = self._check_rows(q, "q")
+        n_seqs, max_pages, pages, hkv, page, cd = self._check_cache(cache, kv_lens, q.dtype)
+        assert n == n_seqs, "q wants one token per sequence"
+        assert cd == d, "q head_dim"
         assert hkv > 0 and hq % hkv == 0, "q heads must be a multiple of k heads"
         if out is None:
-            out = torch.empty((n_seqs, hq, d), dtype=q.dtype, device=q.device)
-        assert out.shape == q.shape and out.dtype == q.dtype, "out shape"
-        self._check_tensor(out, "out")
+            out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        else:
+            self._check_out(out, q, "out")
         if out.numel() == 0:
             return out
         if workspace is None:
             workspace = self.paged_workspace()
-        self._check_tensor(workspace, "workspace")
+        else:
+            self._check_tensor(workspace, "workspace")
         self._bind_stream()
-        check(self._L.hs_attention_paged(self._h, _ptr(q), _ptr(out), _ptr(cache.k), _ptr(cache.v),
-                                         _ptr(cache.block_table), _ptr(kv_lens), qs, n_seqs, hq, hkv, d, pages, page,
-                                         max_pages, _code(q), 0.0 if scale is None else float(scale),
-                                         _ptr(workspace), workspace.numel() * workspace.element_size()))
+        check(self._L.hs_attention_paged(self._h, q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
+                                         cache.block_table.data_ptr(), kv_lens.data_ptr(), qs, n, hq, hkv, d, pages,
+                                         page, max_pages, _code(q), 0.0 if scale is None else scale,
+                                         workspace.data_ptr(), workspace.nbytes))
         return out
 
     _EPILOGUES = {"none": 0, "gelu": 1, "residual_ls": 2}
