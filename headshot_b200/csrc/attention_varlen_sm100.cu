@@ -42,34 +42,53 @@ namespace hs {
 namespace {
 
 constexpr int kBM = 128;  // query rows per tile / softmax warpgroup
-constexpr int kItemSlots = 4;
-constexpr int kItemReaders = 8 + 2;
+constexpr int kItemReaders = 8 + 2 + 1;  // one arrival per softmax warp, per MMA warp and from the producer
 constexpr int kThreads = 384;
 constexpr uint32_t kLaunchRegs = 168;  // 65536 / 384 rounded down to a multiple of 8
-constexpr uint32_t kSoftmaxRegs = 224;
-constexpr uint32_t kControlRegs = 56;
+constexpr uint32_t kSoftmaxRegs = 216;
+constexpr uint32_t kControlRegs = 72;
 static_assert(2 * kSoftmaxRegs + kControlRegs <= 3 * kLaunchRegs, "setmaxnreg split exceeds the launch budget");
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp0 = 9;
-constexpr int kTmemWarp = 11;
+constexpr int kSchedWarp = 11;  // items; also the TMEM owner
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: p <= 2^8 between rescales
 
+#ifndef EMU64
+#define EMU64 2
+#endif
+#ifndef EMU128
+#define EMU128 1
+#endif
+#ifndef PSPLIT
+#define PSPLIT 1
+#endif
+// Head_dim 64: 96-key tiles, two score buffers per warpgroup; a ring slot is a
+// tile's K and V.  Head_dim 128: 128-key tiles, one score buffer; a slot is K or V.
 template <int D>
 struct Shape {
+#ifndef ONE128
   static constexpr int kBN = D == 64 ? 96 : 64;
+  static constexpr int kSBufs = 2;
+  static constexpr int kPParts = 1;
+#else
+  static constexpr int kBN = D == 64 ? 96 : 128;
+  static constexpr int kSBufs = D == 64 ? 2 : 1;
+  static constexpr int kPParts = D == 64 ? 1 : 1 + PSPLIT;
+#endif
   static constexpr int kPairs = kBN / 2;
-  static constexpr int kStages = D == 64 ? 6 : 5;
+  static constexpr int kSlots = D == 64 ? 6 : 5;
   static constexpr int kQBufs = D == 64 ? 2 : 1;
   static constexpr int kHalves = D / 64;             // 128-byte column blocks of a row
   static constexpr int kQTileBytes = kBM * D * 2;
   static constexpr int kKvTileBytes = kBN * D * 2;
+  static constexpr int kSlotBytes = kSBufs * kKvTileBytes;
   static constexpr uint32_t kQHalf = kBM * 128;      // bytes from one column block to the next
   static constexpr uint32_t kKvHalf = kBN * 128;
-  static constexpr int kEmuPer8 = 2;  // of every 8 exponential pairs, this many run on the FMA pipe
-  __host__ __device__ static constexpr uint32_t col_s(int wg, int buf) { return static_cast<uint32_t>((2 * wg + buf) * kBN); }
-  __host__ __device__ static constexpr uint32_t col_o(int wg) { return static_cast<uint32_t>(4 * kBN + D * wg); }
-  static_assert(4 * kBN + 2 * D <= 512, "TMEM budget");
+  static constexpr int kEmuPer8 = D == 64 ? EMU64 : EMU128;  // of every 8 exponential pairs, this many run on the FMA pipe
+  __host__ __device__ static constexpr uint32_t col_s(int wg, int buf) { return static_cast<uint32_t>((kSBufs * wg + buf) * kBN); }
+  __host__ __device__ static constexpr uint32_t col_o(int wg) { return static_cast<uint32_t>(2 * kSBufs * kBN + D * wg); }
+  static_assert(2 * kSBufs * kBN + 2 * D <= 512, "TMEM budget");
   static_assert(kKvHalf % 1024 == 0, "swizzle atoms stay 1024-byte aligned");
 };
 
@@ -106,20 +125,20 @@ constexpr int kNoItem = -1;
 template <int D>
 struct Ctrl {
   using S = Shape<D>;
-  uint64_t kv_full[S::kStages];
-  uint64_t kv_empty[S::kStages];
+  uint64_t kv_full[S::kSlots];
+  uint64_t kv_empty[S::kSlots];
   uint64_t q_full[2][S::kQBufs];
   uint64_t q_empty[2][S::kQBufs];
   uint64_t s_full[2][2];
-  uint64_t p_full[2][2];
+  uint64_t p_full[2][2];  // two score buffers: [buf]; one: the part of P written
   uint64_t pv_prev[2];
   uint64_t pv_last[2];
   uint64_t drain[2];
-  uint64_t item_full[kItemSlots];
-  uint64_t item_empty[kItemSlots];
+  uint64_t item_full;   // the next item is there
+  uint64_t item_empty;  // every reader took it
   uint64_t next_full;
   uint4 next;  // try_cancel's answer
-  Item item[kItemSlots];
+  Item item;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -127,7 +146,7 @@ struct Ctrl {
 template <int D>
 constexpr size_t smem_bytes() {
   using S = Shape<D>;
-  return 1024 + 2 * S::kQBufs * S::kQTileBytes + 2 * S::kStages * S::kKvTileBytes + sizeof(Ctrl<D>);
+  return 1024 + 2 * S::kQBufs * S::kQTileBytes + S::kSlots * S::kSlotBytes + sizeof(Ctrl<D>);
 }
 static_assert(smem_bytes<64>() <= 232448 && smem_bytes<128>() <= 232448, "shared memory per CTA");
 
@@ -147,13 +166,13 @@ struct Args {
 
 __device__ __forceinline__ float u2f(uint32_t u) { return __uint_as_float(u); }
 
-template <int kStages>
+template <int kSlots>
 struct RingPos {
-  uint32_t stage = 0;
+  uint32_t slot = 0;
   uint32_t phase = 0;
   __device__ __forceinline__ void next() {
-    if (++stage == kStages) {
-      stage = 0;
+    if (++slot == kSlots) {
+      slot = 0;
       phase ^= 1;
     }
   }
@@ -173,14 +192,11 @@ __device__ __forceinline__ void mbar_arrive_elect(uint64_t* bar) {
       : "memory");
 }
 
-// Next item for a reader warp (all lanes), from slot k % kItemSlots.
+// Item k for a reader warp (all lanes).
 template <int D>
 __device__ __forceinline__ bool next_item(const Args& a, Ctrl<D>* ctl, uint32_t k, Item* item) {
-  const uint32_t slot = k % kItemSlots;
-  if (!warp_wait(&ctl->item_full[slot], (k / kItemSlots) & 1, &ctl->abort_flag, a.status, kSiteItemFull,
-                 a.timeout_ns))
-    return false;
-  const volatile Item* src = &ctl->item[slot];
+  if (!warp_wait(&ctl->item_full, k & 1, &ctl->abort_flag, a.status, kSiteItemFull, a.timeout_ns)) return false;
+  const volatile Item* src = &ctl->item;
   item->q_row = src->q_row;
   item->tokens = src->tokens;
   item->k_row = src->k_row;
@@ -189,7 +205,7 @@ __device__ __forceinline__ bool next_item(const Args& a, Ctrl<D>* ctl, uint32_t 
   item->head = src->head;
   item->n = src->n;
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(&ctl->item_empty[slot]);
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&ctl->item_empty);
   return true;
 }
 
@@ -249,7 +265,9 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
   // Completions seen before the item: bits of s_full[0], s_full[1], pv_last,
   // pv_prev parities.
   uint32_t base_bits = 0;
-  auto s_parity = [&](uint32_t t) { return ((base_bits >> (t & 1)) + (t >> 1)) & 1; };
+  auto s_parity = [&](uint32_t t) {
+    return S::kSBufs == 2 ? ((base_bits >> (t & 1)) + (t >> 1)) & 1 : (base_bits + t) & 1;
+  };
 
   Item nxt{};
   bool have_nxt = false;
@@ -274,7 +292,7 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
 
     float m_run = -INFINITY, l = 0.f;
     for (uint32_t j = 0; j < n; ++j) {
-      const int b = static_cast<int>(j & 1);
+      const int b = S::kSBufs == 2 ? static_cast<int>(j & 1) : 0;
       if (!warp_wait(&ctl->s_full[wg][b], s_parity(j), abort_flag, a.status, kSiteSFull, a.timeout_ns)) return;
       tc_fence_after();
       const uint32_t tS = tmem + lane_base + S::col_s(wg, b);
@@ -303,6 +321,33 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
         l *= factor;
         need = true;
       }
+      // O rescale (rare), once PV(j-1) has landed.  One score buffer: it was
+      // committed with S(j).  Two: with S(j+1) when that tile exists, else
+      // (j = n-1) as the item's first PV-only batch.
+      auto rescale = [&]() -> bool {
+        if (S::kSBufs == 2) {
+          const bool ok = (j + 1 < n) ? warp_wait(&ctl->s_full[wg][(j + 1) & 1], s_parity(j + 1), abort_flag, a.status,
+                                                  kSiteODone, a.timeout_ns)
+                                      : warp_wait(&ctl->pv_prev[wg], (base_bits >> 3) & 1, abort_flag, a.status,
+                                                  kSiteODone, a.timeout_ns);
+          if (!ok) return false;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int h = 0; h < D / 16; ++h) {  // 16 columns at a time: the scores stay in registers
+          uint32_t o[16];
+          tmem_ld16(tO + 16 * h, o);
+          tmem_wait_ld_regs<16>(o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(u2f(o[i]) * factor);
+          tmem_st16(tO + 16 * h, o);
+        }
+        return true;
+      };
+      // With P handed over in parts the first PV steps start before the tile's
+      // end, so O is rescaled first.
+      const bool any_need = __any_sync(0xffffffffu, need);
+      if (S::kPParts > 1 && any_need && !rescale()) return;
       // A row that sees no key has m_run = -inf and turns into NaN here: its
       // output is set to zero below, and no other row reads it.
       const float neg_m = -m_run;
@@ -319,34 +364,28 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
           p1 = ex2_approx(x1);
         }
         pk[i] = Elem<E>::pack2(p0, p1);
+#ifdef RSUM
         Elem<E>::acc2(acc[2 * (i & 1)], acc[2 * (i & 1) + 1], pk[i]);
-        if (i == 31) tmem_st32(tS, pk);
-      }
-      if constexpr (S::kPairs == 48) tmem_st16(tS + 32, pk + 32);
-      l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-      // O rescale (rare), once PV(j-1) has landed: committed with S(j+1) when
-      // that tile exists, else (j = n-1) as the item's first PV-only batch.
-      if (__any_sync(0xffffffffu, need)) {
-        const bool ok = (j + 1 < n) ? warp_wait(&ctl->s_full[wg][(j + 1) & 1], s_parity(j + 1), abort_flag, a.status,
-                                                kSiteODone, a.timeout_ns)
-                                    : warp_wait(&ctl->pv_prev[wg], (base_bits >> 3) & 1, abort_flag, a.status,
-                                                kSiteODone, a.timeout_ns);
-        if (!ok) return;
-        tc_fence_after();
-#pragma unroll
-        for (int h = 0; h < D / 32; ++h) {
-          uint32_t o[32];
-          tmem_ld32(tO + 32 * h, o);
-          tmem_wait_ld_regs<32>(o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(u2f(o[i]) * factor);
-          tmem_st32(tO + 32 * h, o);
+#else
+        add2(acc[2 * (i & 1)], acc[2 * (i & 1) + 1], acc[2 * (i & 1)], acc[2 * (i & 1) + 1], p0, p1);
+#endif
+        if (i % 32 == 31) {
+          tmem_st32(tS + i - 31, pk + i - 31);
+          if (S::kPParts > 1 && i + 1 < S::kPairs) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_full[wg][0]);
+          }
         }
       }
+      if constexpr (S::kPairs % 32 == 16) tmem_st16(tS + S::kPairs - 16, pk + S::kPairs - 16);
+      l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      if (S::kPParts == 1 && any_need && !rescale()) return;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->p_full[wg][b]);
+      if (lane == 0) mbar_arrive(&ctl->p_full[wg][S::kPParts - 1 + b]);
     }
 
     // The next item's hand-off while PV(n-1) runs.
@@ -355,7 +394,10 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
     if (n > 0) {
       if (!warp_wait(&ctl->pv_last[wg], (base_bits >> 2) & 1, abort_flag, a.status, kSiteODone, a.timeout_ns)) return;
       tc_fence_after();
-      base_bits ^= (((n + 1) >> 1) & 1) | (((n >> 1) & 1) << 1) | 4u | (n > 1 ? 8u : 0u);
+      if (S::kSBufs == 2)
+        base_bits ^= (((n + 1) >> 1) & 1) | (((n >> 1) & 1) << 1) | 4u | (n > 1 ? 8u : 0u);
+      else
+        base_bits ^= (n & 1) | 4u;
     }
     const float inv_l = 1.0f / l;
     const bool empty = lim < 0;
@@ -385,98 +427,120 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
   }
 }
 
-// Items are numbered sequence by sequence, key head by key head, and within
-// one from its last tokens to its first (the longest causal rows first).
+// Items are numbered from costly to cheap, so that the last ones to start are
+// short: by classes of their key count (64 << c, each twice the next), within
+// a class sequence by sequence, last tokens first, and the key heads of the
+// same tokens side by side (one causal prompt of 4,096 tokens, 32/8 x 128, in
+// sequence order head by head: a third of the SM time idle).
 struct Decoder {
-  uint32_t seq0 = 0;    // sequences before it are scanned
-  uint64_t before = 0;  // items of them
+  int cls = 0;          // classes above it are done
+  uint32_t seq0 = 0;    // and in it the sequences before seq0,
+  uint32_t before = 0;  // with this many items in all
 };
 
-// The whole producer warp decodes item number `id`; false: past the last one.
+// Lengths of sequence s, zero if its offsets are out of order or range.
+__device__ __forceinline__ void seq_of(const Args& a, uint32_t s, int* q0, int* lq, int* k0, int* lk) {
+  *q0 = *lq = *k0 = *lk = 0;
+  if (s >= a.n_seqs) return;
+  const int q = __ldg(a.cu_q + s), q1 = __ldg(a.cu_q + s + 1), k = __ldg(a.cu_k + s), k1 = __ldg(a.cu_k + s + 1);
+  if (q < 0 || q1 < q || k < 0 || k1 < k || q1 > static_cast<int>(a.total_q) || k1 > static_cast<int>(a.total_k)) {
+    atomicCAS(a.status, 0, static_cast<int>(kSiteBadOffsets));
+    return;
+  }
+  *q0 = q;
+  *lq = q1 - q;
+  *k0 = k;
+  *lk = k1 - k;
+}
+
+// Items of a sequence (of n) with at most `keys` keys: its first ones.
+__device__ __forceinline__ int items_within(const Args& a, int n, int lq, int lk, int keys, int item_tokens) {
+  if (lk <= keys) return n;
+  if (!a.causal) return 0;
+  return max(0, (keys - (lk - lq)) / item_tokens);
+}
+
+// Whole warp.  Decodes item number `id`; false: past the last one.
 template <int D>
 __device__ __forceinline__ bool decode_item(const Args& a, Decoder& d, uint32_t id, Item* it) {
   const uint32_t lane = threadIdx.x & 31;
   const int item_tokens = 2 * static_cast<int>(a.tile_tokens);
-  if (id < d.before) d = Decoder{};
-  for (; d.seq0 < a.n_seqs; d.seq0 += 32) {
-    const uint32_t s = d.seq0 + lane;
-    int q0 = 0, lq = 0, k0 = 0, lk = 0;
-    if (s < a.n_seqs) {
-      q0 = __ldg(a.cu_q + s);
-      k0 = __ldg(a.cu_k + s);
-      const int q1 = __ldg(a.cu_q + s + 1), k1 = __ldg(a.cu_k + s + 1);
-      if (q0 < 0 || q1 < q0 || k0 < 0 || k1 < k0 || q1 > static_cast<int>(a.total_q) ||
-          k1 > static_cast<int>(a.total_k)) {
-        atomicCAS(a.status, 0, static_cast<int>(kSiteBadOffsets));
-      } else {
-        lq = q1 - q0;
-        lk = k1 - k0;
-      }
-    }
-    const uint32_t tiles = static_cast<uint32_t>((static_cast<int64_t>(lq) + item_tokens - 1) / item_tokens);
-    uint64_t inc = static_cast<uint64_t>(tiles) * a.kv_heads;
-    const uint64_t mine = inc;
+  for (; d.cls >= 0; --d.cls, d.seq0 = 0) {
+    for (; d.seq0 < a.n_seqs; d.seq0 += 32) {
+      int q0, lq, k0, lk;
+      seq_of(a, d.seq0 + lane, &q0, &lq, &k0, &lk);
+      const int n = static_cast<int>((static_cast<uint32_t>(lq) + item_tokens - 1) / item_tokens);
+      const int high = items_within(a, n, lq, lk, d.cls >= 25 ? 0x7fffffff : 64 << d.cls, item_tokens);
+      const int low = d.cls > 0 ? items_within(a, n, lq, lk, 32 << d.cls, item_tokens) : 0;
+      const uint32_t mine = static_cast<uint32_t>(high - low) * a.kv_heads;
+      uint32_t inc = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= static_cast<uint32_t>(o)) inc += up;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= static_cast<uint32_t>(o)) inc += up;
+      }
+      const uint32_t local = id - (d.before + inc - mine);
+      const uint32_t hit = __ballot_sync(0xffffffffu, local < mine);
+      if (!hit) {
+        d.before += __shfl_sync(0xffffffffu, inc, 31);
+        continue;
+      }
+      const int src = __ffs(hit) - 1;
+      const int t0 = (high - 1 - static_cast<int>(local / a.kv_heads)) * item_tokens;
+      it->head = __shfl_sync(0xffffffffu, local % a.kv_heads, src);
+      it->q_row = __shfl_sync(0xffffffffu, q0 + t0, src);
+      it->tokens = __shfl_sync(0xffffffffu, lq - t0, src);
+      it->k_row = __shfl_sync(0xffffffffu, k0, src);
+      it->n_keys = __shfl_sync(0xffffffffu, lk, src);
+      it->lim = __shfl_sync(0xffffffffu, t0 + lk - lq, src);
+      it->n = max(wg_tiles<D>(a, *it, 0), wg_tiles<D>(a, *it, 1));
+      return true;
     }
-    const uint64_t first = d.before + inc - mine;
-    const uint32_t hit = __ballot_sync(0xffffffffu, id >= first && id < first + mine);
-    if (!hit) {
-      d.before += __shfl_sync(0xffffffffu, inc, 31);
-      continue;
-    }
-    const int src = __ffs(hit) - 1;
-    const uint32_t local = static_cast<uint32_t>(id - __shfl_sync(0xffffffffu, first, src));
-    const uint32_t n = __shfl_sync(0xffffffffu, tiles, src);
-    q0 = __shfl_sync(0xffffffffu, q0, src);
-    lq = __shfl_sync(0xffffffffu, lq, src);
-    k0 = __shfl_sync(0xffffffffu, k0, src);
-    lk = __shfl_sync(0xffffffffu, lk, src);
-    it->head = local / n;
-    const int t0 = static_cast<int>(n - 1 - local % n) * item_tokens;
-    it->q_row = q0 + t0;
-    it->tokens = lq - t0;
-    it->k_row = k0;
-    it->n_keys = lk;
-    it->lim = t0 + lk - lq;
-    it->n = max(wg_tiles<D>(a, *it, 0), wg_tiles<D>(a, *it, 1));
-    return true;
   }
   return false;
 }
 
-// The producer warp, converged: lane 0 issues.
+// The scheduler warp, converged: decodes this block's item, then the items of
+// the pending blocks it takes over, one ahead of the readers.
 template <int D>
-__device__ void producer_role(const Args& a, const CUtensorMap* tm_q, const CUtensorMap* tm_k,
-                              const CUtensorMap* tm_v, uint8_t* sQ, uint8_t* sK, uint8_t* sV, Ctrl<D>* ctl) {
-  using S = Shape<D>;
+__device__ void scheduler_role(const Args& a, Ctrl<D>* ctl) {
   volatile int* abort_flag = &ctl->abort_flag;
   const bool lead = (threadIdx.x & 31) == 0;
-  uint32_t q_issued[2] = {0, 0};
-  uint32_t g = 0;     // K/V tiles issued so far
-  uint32_t k = 0;     // items posted
-  uint32_t asked = 0; // try_cancel requests
-  bool ok = true;
-  Decoder dec;
-  uint32_t id = blockIdx.x;
-  const uint32_t q_bytes = a.tile_tokens * a.group * 128 * S::kHalves;
+  uint32_t k = 0;      // items posted
+  uint32_t asked = 0;  // try_cancel requests
+  // The class of the longest key run.
+  int most = 0;
+  for (uint32_t s = threadIdx.x & 31; s < a.n_seqs; s += 32) {
+    int q0, lq, k0, lk;
+    seq_of(a, s, &q0, &lq, &k0, &lk);
+    most = max(most, lk);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const int top = most > 64 ? 26 - __clz(most - 1) : 0;  // smallest c with most <= 64 << c
+  Decoder dec{top, 0, 0};
   auto post = [&](const Item& it) {
-    const uint32_t slot = k % kItemSlots;
-    if (k >= kItemSlots && !warp_wait(&ctl->item_empty[slot], ((k / kItemSlots) - 1) & 1, abort_flag, a.status,
-                                      kSiteItemEmpty, a.timeout_ns))
+    if (k > 0 &&
+        !warp_wait(&ctl->item_empty, (k - 1) & 1, abort_flag, a.status, kSiteItemEmpty, a.timeout_ns))
       return false;
     if (lead) {
-      ctl->item[slot] = it;
-      mbar_arrive(&ctl->item_full[slot]);  // release: visible to the readers' acquire
+      ctl->item = it;
+      mbar_arrive(&ctl->item_full);  // release: visible to the readers' acquire
     }
     __syncwarp();
     ++k;
     return true;
   };
+  uint32_t id = blockIdx.x, last = 0;
+  bool ok = true;
   while (true) {
-    // Ask for the next pending block; the answer is read after this item's loads.
+    if (id < last) dec = Decoder{top, 0, 0};
+    last = id;
+    Item it;
+    if (decode_item<D>(a, dec, id, &it) && !post(it)) {
+      ok = false;
+      break;
+    }
     if (lead) {
       mbar_arrive_expect_tx(&ctl->next_full, 16);
       asm volatile(
@@ -486,53 +550,6 @@ __device__ void producer_role(const Args& a, const CUtensorMap* tm_q, const CUte
           : "memory");
     }
     ++asked;
-    Item it;
-    if (decode_item<D>(a, dec, id, &it)) {
-      if (!post(it)) {
-        ok = false;
-        break;
-      }
-#pragma unroll
-      for (int wg = 0; wg < 2; ++wg) {
-        if (!ok || wg_tiles<D>(a, it, wg) == 0) continue;
-        const uint32_t qi = q_issued[wg];
-        const uint32_t qb = qi % S::kQBufs;
-        if (qi >= S::kQBufs && !warp_wait(&ctl->q_empty[wg][qb], ((qi / S::kQBufs) - 1) & 1, abort_flag, a.status,
-                                          kSiteQEmpty, a.timeout_ns)) {
-          ok = false;
-          continue;
-        }
-        if (lead) {
-          mbar_arrive_expect_tx(&ctl->q_full[wg][qb], q_bytes);
-#pragma unroll
-          for (int h = 0; h < S::kHalves; ++h)
-            tma_load_4d(tm_q, &ctl->q_full[wg][qb], sQ + (wg * S::kQBufs + qb) * S::kQTileBytes + h * S::kQHalf,
-                        64 * h, 0, static_cast<int>(it.head), it.q_row + wg * static_cast<int>(a.tile_tokens));
-        }
-        q_issued[wg] = qi + 1;
-      }
-      for (uint32_t j = 0; ok && j < it.n; ++j, ++g) {
-        const uint32_t st = g % S::kStages;
-        if (g >= S::kStages && !warp_wait(&ctl->kv_empty[st], ((g / S::kStages) - 1) & 1, abort_flag, a.status,
-                                          kSiteKvEmpty, a.timeout_ns)) {
-          ok = false;
-          break;
-        }
-        if (lead) {
-          const int key = it.k_row + static_cast<int>(j) * S::kBN;
-          mbar_arrive_expect_tx(&ctl->kv_full[st], 2 * S::kKvTileBytes);
-#pragma unroll
-          for (int h = 0; h < S::kHalves; ++h)
-            tma_load_3d(tm_k, &ctl->kv_full[st], sK + st * S::kKvTileBytes + h * S::kKvHalf, 64 * h,
-                        static_cast<int>(it.head), key);
-#pragma unroll
-          for (int h = 0; h < S::kHalves; ++h)
-            tma_load_3d(tm_v, &ctl->kv_full[st], sV + st * S::kKvTileBytes + h * S::kKvHalf, 64 * h,
-                        static_cast<int>(it.head), key);
-        }
-      }
-      if (!ok) break;
-    }
     if (!warp_wait(&ctl->next_full, (asked - 1) & 1, abort_flag, a.status, kSiteNext, a.timeout_ns)) {
       ok = false;
       break;
@@ -554,10 +571,72 @@ __device__ void producer_role(const Args& a, const CUtensorMap* tm_q, const CUte
     id = x;
   }
   if (ok) post(Item{kNoItem, 0, 0, 0, 0, 0, 0});
-  // Every copy and answer this warp asked for lands before the CTA can exit.
-  mbar_wait_teardown(&ctl->next_full, (asked - 1) & 1, a.status, kSiteNext);
-  for (uint32_t t = g > S::kStages ? g - S::kStages : 0; t < g; ++t)
-    mbar_wait_teardown(&ctl->kv_full[t % S::kStages], (t / S::kStages) & 1, a.status, kSiteKvFull);
+  // The answer to every request lands before the CTA can exit.
+  if (asked) mbar_wait_teardown(&ctl->next_full, (asked - 1) & 1, a.status, kSiteNext);
+  __syncwarp();
+}
+
+// The producer warp, converged: lane 0 issues.
+template <int D>
+__device__ void producer_role(const Args& a, const CUtensorMap* tm_q, const CUtensorMap* tm_k,
+                              const CUtensorMap* tm_v, uint8_t* sQ, uint8_t* sKv, Ctrl<D>* ctl) {
+  using S = Shape<D>;
+  volatile int* abort_flag = &ctl->abort_flag;
+  const bool lead = (threadIdx.x & 31) == 0;
+  uint32_t q_issued[2] = {0, 0};
+  uint32_t g = 0;  // ring slots filled so far
+  bool ok = true;
+  const uint32_t q_bytes = a.tile_tokens * a.group * 128 * S::kHalves;
+  for (uint32_t k = 0; ok; ++k) {
+    Item it;
+    if (!next_item<D>(a, ctl, k, &it) || it.q_row == kNoItem) break;
+#pragma unroll
+    for (int wg = 0; wg < 2; ++wg) {
+      if (!ok || wg_tiles<D>(a, it, wg) == 0) continue;
+      const uint32_t qi = q_issued[wg];
+      const uint32_t qb = qi % S::kQBufs;
+      if (qi >= S::kQBufs && !warp_wait(&ctl->q_empty[wg][qb], ((qi / S::kQBufs) - 1) & 1, abort_flag, a.status,
+                                        kSiteQEmpty, a.timeout_ns)) {
+        ok = false;
+        continue;
+      }
+      if (lead) {
+        mbar_arrive_expect_tx(&ctl->q_full[wg][qb], q_bytes);
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h)
+          tma_load_4d(tm_q, &ctl->q_full[wg][qb], sQ + (wg * S::kQBufs + qb) * S::kQTileBytes + h * S::kQHalf,
+                      64 * h, 0, static_cast<int>(it.head), it.q_row + wg * static_cast<int>(a.tile_tokens));
+      }
+      q_issued[wg] = qi + 1;
+    }
+    for (uint32_t j = 0; ok && j < it.n; ++j) {
+      const int key = it.k_row + static_cast<int>(j) * S::kBN;
+      // K and V of the tile, in one slot or in two.
+#pragma unroll
+      for (int part = 0; part < 3 - S::kSBufs; ++part) {
+        const uint32_t st = g % S::kSlots;
+        if (g >= S::kSlots && !warp_wait(&ctl->kv_empty[st], ((g / S::kSlots) - 1) & 1, abort_flag, a.status,
+                                         kSiteKvEmpty, a.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        if (lead) {
+          uint8_t* slot = sKv + st * S::kSlotBytes;
+          mbar_arrive_expect_tx(&ctl->kv_full[st], S::kSlotBytes);
+#pragma unroll
+          for (int t = 0; t < S::kSBufs; ++t)
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+              tma_load_3d(part + t ? tm_v : tm_k, &ctl->kv_full[st], slot + t * S::kKvTileBytes + h * S::kKvHalf,
+                          64 * h, static_cast<int>(it.head), key);
+        }
+        ++g;
+      }
+    }
+  }
+  // Every copy this warp asked for lands before the CTA can exit.
+  for (uint32_t t = g > S::kSlots ? g - S::kSlots : 0; t < g; ++t)
+    mbar_wait_teardown(&ctl->kv_full[t % S::kSlots], (t / S::kSlots) & 1, a.status, kSiteKvFull);
 #pragma unroll
   for (int wg = 0; wg < 2; ++wg) {
     const uint32_t qi = q_issued[wg];
@@ -569,7 +648,7 @@ __device__ void producer_role(const Args& a, const CUtensorMap* tm_q, const CUte
 
 // One MMA warp per softmax warpgroup, converged; elect.sync issues.
 template <typename E, int D>
-__device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sK, uint8_t* sV, Ctrl<D>* ctl, uint32_t tmem) {
+__device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sKv, Ctrl<D>* ctl, uint32_t tmem) {
   using S = Shape<D>;
   constexpr int kBN = S::kBN;
   volatile int* abort_flag = &ctl->abort_flag;
@@ -580,39 +659,45 @@ __device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sK, uint8_
   // block, then to the next block; a 16-key step of V advances by 2048 B, and
   // V's second block of 64 columns lies a leading-dimension stride on.
   const uint64_t q_desc0 = sdesc_sw128(smem_u32(sQ + wg * S::kQBufs * S::kQTileBytes), 16, 1024);
-  const uint64_t k_desc = sdesc_sw128(smem_u32(sK), 16, 1024);
-  const uint64_t v_desc = sdesc_sw128(smem_u32(sV), S::kKvHalf, 1024);
-  constexpr uint64_t kKvTileStep = S::kKvTileBytes >> 4;
+  // A slot's K is at its start, its V behind K where the two share a slot.
+  constexpr uint32_t kVOffset = (S::kSBufs - 1) * S::kKvTileBytes;
+  const uint64_t k_desc = sdesc_sw128(smem_u32(sKv), 16, 1024);
+  const uint64_t v_desc = sdesc_sw128(smem_u32(sKv) + kVOffset, S::kKvHalf, 1024);
+  constexpr uint64_t kSlotStep = S::kSlotBytes >> 4;
   constexpr uint64_t kQTileStep = S::kQTileBytes >> 4;
   const uint32_t o_tmem = tmem + S::col_o(wg);
   uint32_t p_base0 = 0, p_base1 = 0;  // p_full completions before this item, per buffer
   uint32_t q_used = 0;
-  RingPos<S::kStages> s_pos;   // next K/V tile to wait for (S products, or release)
-  RingPos<S::kStages> pv_pos;  // next K/V tile whose V feeds a PV product
+  RingPos<S::kSlots> s_pos;   // next slot to wait for (two score buffers: K and V of a tile)
+  RingPos<S::kSlots> pv_pos;  // two score buffers: next slot whose V feeds a PV product
   bool ok = true;
 
   auto issue_s = [&](uint64_t q_desc, uint32_t st, int buf) {
-    const uint64_t kd = k_desc + st * kKvTileStep;
+    const uint64_t kd = k_desc + st * kSlotStep;
     const uint32_t d = tmem + S::col_s(wg, buf);
 #pragma unroll
     for (int k = 0; k < D / 16; ++k)
       umma_ss_elect(d, q_desc + (k >> 2) * (S::kQHalf >> 4) + 2 * (k & 3), kd + (k >> 2) * (S::kKvHalf >> 4) + 2 * (k & 3),
                     idesc_qk, k > 0 ? 1u : 0u);
   };
-  auto issue_pv = [&](uint32_t st, int buf, bool acc) {
-    const uint64_t vd = v_desc + st * kKvTileStep;
+  // Part `part` of the tile's PV product (of kPParts).
+  auto issue_pv = [&](uint32_t st, int buf, int part, bool acc) {
+    const uint64_t vd = v_desc + st * kSlotStep;
     const uint32_t p = tmem + S::col_s(wg, buf);
+    constexpr int kSteps = kBN / 16 / S::kPParts;
 #pragma unroll
-    for (int k = 0; k < kBN / 16; ++k)
+    for (int x = 0; x < kSteps; ++x) {
+      const int k = part * kSteps + x;
       umma_ts_elect(o_tmem, p + 8 * k, vd + 128 * k, idesc_pv, (acc || k > 0) ? 1u : 0u);
+    }
   };
-  auto kv_wait = [&](const RingPos<S::kStages>& r) {
-    return warp_wait(&ctl->kv_full[r.stage], r.phase, abort_flag, a.status, kSiteKvFull, a.timeout_ns);
+  auto kv_wait = [&](const RingPos<S::kSlots>& r) {
+    return warp_wait(&ctl->kv_full[r.slot], r.phase, abort_flag, a.status, kSiteKvFull, a.timeout_ns);
   };
   // Values behind the sequence's end become zero.  Both MMA warps write the
   // same zeros; a warp's own products are issued behind its fence.
   auto clear_tail = [&](uint32_t st, int keys) {
-    uint8_t* v = sV + st * S::kKvTileBytes;
+    uint8_t* v = sKv + st * S::kSlotBytes + kVOffset;
     const int lane = threadIdx.x & 31;
     for (int x = keys * 8 + lane; x < kBN * 8; x += 32) {
 #pragma unroll
@@ -650,63 +735,108 @@ __device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sK, uint8_
       const uint64_t q_desc = q_desc0 + qb * kQTileStep;
       // Keys of this warpgroup's last tile that belong to the sequence, if not all do.
       const int tail = it.n_keys - static_cast<int>(n - 1) * kBN;
-      // S(0) and S(1) up front.  The commit after the item's last S also frees its Q buffer.
-      for (uint32_t t = 0; t < 2 && t < n; ++t) {
-        if (!kv_wait(s_pos)) {
-          ok = false;
-          break;
-        }
-        issue_s(q_desc, s_pos.stage, static_cast<int>(t));
-        s_pos.next();
-        umma_commit_elect(&ctl->s_full[wg][t]);
-        if (t == n - 1) {
-          umma_commit_elect(&ctl->q_empty[wg][qb]);
-          if (!fetch_next(k + 1)) ok = false;
-        }
-      }
-      for (uint32_t j = 0; ok && j < n; ++j) {
-        const int b = static_cast<int>(j & 1);
-        const uint32_t st = pv_pos.stage;  // V_j: waited on before S(j) was issued
-        pv_pos.next();
-        if (j + 1 == n && tail < kBN) clear_tail(st, tail);
-        if (!warp_wait(&ctl->p_full[wg][b], ((b ? p_base1 : p_base0) + (j >> 1)) & 1, abort_flag, a.status,
-                       kSitePFull, a.timeout_ns)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        issue_pv(st, b, j > 0);
-        if (j + 2 < n) {
+      if constexpr (S::kSBufs == 2) {
+        // S(0) and S(1) up front.  The commit after the item's last S also frees its Q buffer.
+        for (uint32_t t = 0; t < 2 && t < n; ++t) {
           if (!kv_wait(s_pos)) {
             ok = false;
             break;
           }
-          issue_s(q_desc, s_pos.stage, b);  // after PV(j) in this warp's order: P(j) is read first
+          issue_s(q_desc, s_pos.slot, static_cast<int>(t));
           s_pos.next();
-          umma_commit_elect(&ctl->s_full[wg][b]);
-          if (j + 2 == n - 1) {
+          umma_commit_elect(&ctl->s_full[wg][t]);
+          if (t == n - 1) {
             umma_commit_elect(&ctl->q_empty[wg][qb]);
-            if (!fetch_next(k + 1)) {
+            if (!fetch_next(k + 1)) ok = false;
+          }
+        }
+        for (uint32_t j = 0; ok && j < n; ++j) {
+          const int b = static_cast<int>(j & 1);
+          const uint32_t st = pv_pos.slot;  // V_j: waited on before S(j) was issued
+          pv_pos.next();
+          if (j + 1 == n && tail < kBN) clear_tail(st, tail);
+          if (!warp_wait(&ctl->p_full[wg][b], ((b ? p_base1 : p_base0) + (j >> 1)) & 1, abort_flag, a.status,
+                         kSitePFull, a.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          issue_pv(st, b, 0, j > 0);
+          if (j + 2 < n) {
+            if (!kv_wait(s_pos)) {
               ok = false;
               break;
             }
+            issue_s(q_desc, s_pos.slot, b);  // after PV(j) in this warp's order: P(j) is read first
+            s_pos.next();
+            umma_commit_elect(&ctl->s_full[wg][b]);
+            if (j + 2 == n - 1) {
+              umma_commit_elect(&ctl->q_empty[wg][qb]);
+              if (!fetch_next(k + 1)) {
+                ok = false;
+                break;
+              }
+            }
+          } else {
+            umma_commit_elect(j + 1 == n ? &ctl->pv_last[wg] : &ctl->pv_prev[wg]);
           }
-        } else {
-          umma_commit_elect(j + 1 == n ? &ctl->pv_last[wg] : &ctl->pv_prev[wg]);
+          umma_commit_elect(&ctl->kv_empty[st]);
         }
-        umma_commit_elect(&ctl->kv_empty[st]);
+      } else {
+        // S(0); then per tile PV(j) part by part and S(j+1), which overwrites P(j)
+        // behind it.  Slots: K(j), V(j), K(j+1), ...; S(j) frees K(j), PV(j) V(j).
+        for (uint32_t j = 0; ok && j <= n; ++j) {
+          if (j > 0) {  // PV(j-1)
+            const uint32_t t = j - 1;
+            if (!kv_wait(s_pos)) {
+              ok = false;
+              break;
+            }
+            const uint32_t st = s_pos.slot;
+            s_pos.next();
+            if (t + 1 == n && tail < kBN) clear_tail(st, tail);
+  #pragma unroll
+            for (int part = 0; part < S::kPParts; ++part) {
+              if (!warp_wait(&ctl->p_full[wg][part], (p_base0 + t) & 1, abort_flag, a.status, kSitePFull,
+                             a.timeout_ns)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              issue_pv(st, 0, part, t > 0);
+            }
+            if (!ok) break;
+            umma_commit_elect(&ctl->kv_empty[st]);
+          }
+          if (j == n) {
+            umma_commit_elect(&ctl->pv_last[wg]);
+            break;
+          }
+          if (!kv_wait(s_pos)) {
+            ok = false;
+            break;
+          }
+          issue_s(q_desc, s_pos.slot, 0);
+          umma_commit_elect(&ctl->s_full[wg][0]);
+          umma_commit_elect(&ctl->kv_empty[s_pos.slot]);
+          s_pos.next();
+          if (j == n - 1) {
+            umma_commit_elect(&ctl->q_empty[wg][qb]);
+            if (!fetch_next(k + 1)) ok = false;
+          }
+        }
       }
-      p_base0 += (n + 1) >> 1;
+      p_base0 += S::kSBufs == 2 ? (n + 1) >> 1 : n;
       p_base1 += n >> 1;
       ++q_used;
     }
     // Tiles only the other warpgroup needs: released once they have landed.
-    for (uint32_t j = n; ok && j < it.n; ++j, s_pos.next()) {
+    for (uint32_t j = n * (3 - S::kSBufs); ok && j < it.n * (3 - S::kSBufs); ++j, s_pos.next()) {
       if (!kv_wait(s_pos)) {
         ok = false;
         break;
       }
-      mbar_arrive_elect(&ctl->kv_empty[s_pos.stage]);
+      mbar_arrive_elect(&ctl->kv_empty[s_pos.slot]);
     }
     pv_pos = s_pos;
   }
@@ -724,14 +854,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sK = sQ + 2 * S::kQBufs * S::kQTileBytes;
-  uint8_t* sV = sK + S::kStages * S::kKvTileBytes;
-  Ctrl<D>* ctl = reinterpret_cast<Ctrl<D>*>(sV + S::kStages * S::kKvTileBytes);
+  uint8_t* sKv = sQ + 2 * S::kQBufs * S::kQTileBytes;
+  Ctrl<D>* ctl = reinterpret_cast<Ctrl<D>*>(sKv + S::kSlots * S::kSlotBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < S::kSlots; ++s) {
       mbar_init(&ctl->kv_full[s], 1);
       mbar_init(&ctl->kv_empty[s], 2);
     }
@@ -748,10 +877,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl->pv_last[i], 1);
       mbar_init(&ctl->drain[i], 1);
     }
-    for (int i = 0; i < kItemSlots; ++i) {
-      mbar_init(&ctl->item_full[i], 1);
-      mbar_init(&ctl->item_empty[i], kItemReaders);
-    }
+    mbar_init(&ctl->item_full, 1);
+    mbar_init(&ctl->item_empty, kItemReaders);
     mbar_init(&ctl->next_full, 1);
     ctl->abort_flag = 0;
     fence_mbar_init();
@@ -761,7 +888,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  if (warp == kTmemWarp) {
+  if (warp == kSchedWarp) {
     tmem_alloc(&ctl->tmem_base, kTmemCols);
     tmem_relinquish();
   }
@@ -776,14 +903,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     regs_dec<kControlRegs>();
     if (warp == kProducerWarp)
-      producer_role<D>(a, &tm_q, &tm_k, &tm_v, sQ, sK, sV, ctl);
+      producer_role<D>(a, &tm_q, &tm_k, &tm_v, sQ, sKv, ctl);
     else if (warp == kMmaWarp0 || warp == kMmaWarp0 + 1)
-      mma_role<E, D>(a, warp - kMmaWarp0, sQ, sK, sV, ctl, tmem);
+      mma_role<E, D>(a, warp - kMmaWarp0, sQ, sKv, ctl, tmem);
+    else
+      scheduler_role<D>(a, ctl);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == kTmemWarp) {
+  if (warp == kSchedWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
