@@ -14,12 +14,11 @@
 //   by token (one TMA box), so all heads that share keys share the K/V tiles
 //   and a short sequence fills rows with heads.  An item is two such tiles of
 //   one (sequence, key head) against its keys.
-// - The grid covers every item the packed rows can hold; a resident CTA takes
-//   over the next pending one with clusterlaunchcontrol.try_cancel while it
-//   works on the current one.  Scheduling is dynamic without a counter in
-//   memory, so launches share nothing.  Which sequence an item belongs to is
-//   found from the offsets on the device.  Items of a (sequence, key head) go
-//   out longest first, head by head, so the CTAs at work share K/V in L2.
+// - The grid covers every item the packed rows can hold; a scheduler warp takes
+//   over the next pending block with clusterlaunchcontrol.try_cancel while the
+//   CTA works on the current item.  Scheduling is dynamic without a counter in
+//   memory, so launches share nothing, and costly items go out first.  Which
+//   sequence an item belongs to is found from the offsets on the device.
 // - Under a causal mask each warpgroup stops at its own last key tile; tiles
 //   that cross the diagonal or the sequence's end are masked element by element.
 // - The keys of a tile that lie behind the sequence belong to the next one:
@@ -29,8 +28,30 @@
 //
 // Head_dim 64: 96-key tiles; 128: 64-key tiles, since two f32 accumulators of
 // 128 columns leave 256 of TMEM's 512 columns for the four score buffers.
-// Rounding: P is rounded to the storage type for the PV product and the row sum
-// adds the rounded P; statistics and accumulators are f32.
+// Rounding: P is rounded to the storage type for the PV product; statistics,
+// the row sum (of the unrounded P, in packed adds: summing the rounded P costs
+// 3 % of the speed at 128 and 3 % at 64) and accumulators are f32.
+//
+// What bounds it (8,192 tokens, 32/8 x 128, not causal, one burst at 1,965 MHz:
+// 854 us, 1,288 TFLOP/s): per pair of 128 x 64 tiles about 1,900 cycles, of
+// which the tensor core's share is 1,260 (64-column score products run at two
+// thirds of its rate) and the MUFU's 900.  A softmax warp spends 1,070 of them
+// in the exponentials, both warpgroups at the same time and so at half the
+// MUFU's rate each, 290 in the maximum and 220 waiting for scores.  Under load
+// the 1,000 W cap takes the clock to 1,600 MHz: 1,168 TFLOP/s for a causal
+// prompt of 16,384.  Head_dim 64 is bound by the exponentials as
+// attn_fwd_sm100 is: 790 TFLOP/s for 16,384 tokens, 16 x 64, not causal.
+// Built, measured and not kept (8,192 / 16,384 tokens as above, against 1,215
+// and 790 TFLOP/s on the same GPUs):
+//   head_dim 128 with 128-key tiles and one score buffer (1,079; with one MMA
+//     warp for both warpgroups 1,170, without splitting P's hand-over 1,251 in
+//     a burst, 1,052 against 1,141 at the power cap)
+//   one MMA warp for both warpgroups, 64-key tiles (970 / 747)
+//   the warpgroups' exponentials taking turns (1,175 / 720)
+//   each tile's exponentials interleaved with the next one's maximum, three
+//     64-key score buffers at head_dim 64 (806 / 748)
+//   the next K/V tile awaited before P instead of after (1,175 / 768)
+//   four MMAs per election (1,214 / 781 to 801)
 #include <cuda.h>
 
 #include <algorithm>
@@ -54,41 +75,25 @@ constexpr int kSchedWarp = 11;  // items; also the TMEM owner
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: p <= 2^8 between rescales
 
-#ifndef EMU64
-#define EMU64 2
-#endif
-#ifndef EMU128
-#define EMU128 1
-#endif
-#ifndef PSPLIT
-#define PSPLIT 1
-#endif
-// Head_dim 64: 96-key tiles, two score buffers per warpgroup; a ring slot is a
-// tile's K and V.  Head_dim 128: 128-key tiles, one score buffer; a slot is K or V.
 template <int D>
 struct Shape {
-#ifndef ONE128
-  static constexpr int kBN = D == 64 ? 96 : 64;
-  static constexpr int kSBufs = 2;
-  static constexpr int kPParts = 1;
-#else
-  static constexpr int kBN = D == 64 ? 96 : 128;
-  static constexpr int kSBufs = D == 64 ? 2 : 1;
-  static constexpr int kPParts = D == 64 ? 1 : 1 + PSPLIT;
-#endif
+  static constexpr int kBN = D == 64 ? 96 : 64;  // keys per tile: 4 kBN + 2 D columns of TMEM
   static constexpr int kPairs = kBN / 2;
-  static constexpr int kSlots = D == 64 ? 6 : 5;
+  static constexpr int kSlots = D == 64 ? 6 : 5;  // K/V tiles in shared memory
   static constexpr int kQBufs = D == 64 ? 2 : 1;
-  static constexpr int kHalves = D / 64;             // 128-byte column blocks of a row
+  static constexpr int kHalves = D / 64;          // 128-byte column blocks of a row
   static constexpr int kQTileBytes = kBM * D * 2;
   static constexpr int kKvTileBytes = kBN * D * 2;
-  static constexpr int kSlotBytes = kSBufs * kKvTileBytes;
-  static constexpr uint32_t kQHalf = kBM * 128;      // bytes from one column block to the next
+  static constexpr int kSlotBytes = 2 * kKvTileBytes;
+  static constexpr uint32_t kQHalf = kBM * 128;   // bytes from one column block to the next
   static constexpr uint32_t kKvHalf = kBN * 128;
-  static constexpr int kEmuPer8 = D == 64 ? EMU64 : EMU128;  // of every 8 exponential pairs, this many run on the FMA pipe
-  __host__ __device__ static constexpr uint32_t col_s(int wg, int buf) { return static_cast<uint32_t>((kSBufs * wg + buf) * kBN); }
-  __host__ __device__ static constexpr uint32_t col_o(int wg) { return static_cast<uint32_t>(2 * kSBufs * kBN + D * wg); }
-  static_assert(2 * kSBufs * kBN + 2 * D <= 512, "TMEM budget");
+  // Of every 8 exponential pairs, this many run on the FMA pipe.  8,192 tokens
+  // of 32/8 x 128 (0, 1, 2 of 8): 1138, 1168, 1135 TFLOP/s at the power cap;
+  // 16,384 of 16 x 64 (0, 1, 2, 3): 675, 722, 727, 731.
+  static constexpr int kEmuPer8 = D == 64 ? 2 : 1;
+  __host__ __device__ static constexpr uint32_t col_s(int wg, int buf) { return static_cast<uint32_t>((2 * wg + buf) * kBN); }
+  __host__ __device__ static constexpr uint32_t col_o(int wg) { return static_cast<uint32_t>(4 * kBN + D * wg); }
+  static_assert(4 * kBN + 2 * D <= 512, "TMEM budget");
   static_assert(kKvHalf % 1024 == 0, "swizzle atoms stay 1024-byte aligned");
 };
 
@@ -130,7 +135,7 @@ struct Ctrl {
   uint64_t q_full[2][S::kQBufs];
   uint64_t q_empty[2][S::kQBufs];
   uint64_t s_full[2][2];
-  uint64_t p_full[2][2];  // two score buffers: [buf]; one: the part of P written
+  uint64_t p_full[2][2];
   uint64_t pv_prev[2];
   uint64_t pv_last[2];
   uint64_t drain[2];
@@ -265,9 +270,7 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
   // Completions seen before the item: bits of s_full[0], s_full[1], pv_last,
   // pv_prev parities.
   uint32_t base_bits = 0;
-  auto s_parity = [&](uint32_t t) {
-    return S::kSBufs == 2 ? ((base_bits >> (t & 1)) + (t >> 1)) & 1 : (base_bits + t) & 1;
-  };
+  auto s_parity = [&](uint32_t t) { return ((base_bits >> (t & 1)) + (t >> 1)) & 1; };
 
   Item nxt{};
   bool have_nxt = false;
@@ -292,7 +295,7 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
 
     float m_run = -INFINITY, l = 0.f;
     for (uint32_t j = 0; j < n; ++j) {
-      const int b = S::kSBufs == 2 ? static_cast<int>(j & 1) : 0;
+      const int b = static_cast<int>(j & 1);
       if (!warp_wait(&ctl->s_full[wg][b], s_parity(j), abort_flag, a.status, kSiteSFull, a.timeout_ns)) return;
       tc_fence_after();
       const uint32_t tS = tmem + lane_base + S::col_s(wg, b);
@@ -321,33 +324,6 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
         l *= factor;
         need = true;
       }
-      // O rescale (rare), once PV(j-1) has landed.  One score buffer: it was
-      // committed with S(j).  Two: with S(j+1) when that tile exists, else
-      // (j = n-1) as the item's first PV-only batch.
-      auto rescale = [&]() -> bool {
-        if (S::kSBufs == 2) {
-          const bool ok = (j + 1 < n) ? warp_wait(&ctl->s_full[wg][(j + 1) & 1], s_parity(j + 1), abort_flag, a.status,
-                                                  kSiteODone, a.timeout_ns)
-                                      : warp_wait(&ctl->pv_prev[wg], (base_bits >> 3) & 1, abort_flag, a.status,
-                                                  kSiteODone, a.timeout_ns);
-          if (!ok) return false;
-          tc_fence_after();
-        }
-#pragma unroll
-        for (int h = 0; h < D / 16; ++h) {  // 16 columns at a time: the scores stay in registers
-          uint32_t o[16];
-          tmem_ld16(tO + 16 * h, o);
-          tmem_wait_ld_regs<16>(o);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(u2f(o[i]) * factor);
-          tmem_st16(tO + 16 * h, o);
-        }
-        return true;
-      };
-      // With P handed over in parts the first PV steps start before the tile's
-      // end, so O is rescaled first.
-      const bool any_need = __any_sync(0xffffffffu, need);
-      if (S::kPParts > 1 && any_need && !rescale()) return;
       // A row that sees no key has m_run = -inf and turns into NaN here: its
       // output is set to zero below, and no other row reads it.
       const float neg_m = -m_run;
@@ -364,28 +340,34 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
           p1 = ex2_approx(x1);
         }
         pk[i] = Elem<E>::pack2(p0, p1);
-#ifdef RSUM
-        Elem<E>::acc2(acc[2 * (i & 1)], acc[2 * (i & 1) + 1], pk[i]);
-#else
         add2(acc[2 * (i & 1)], acc[2 * (i & 1) + 1], acc[2 * (i & 1)], acc[2 * (i & 1) + 1], p0, p1);
-#endif
-        if (i % 32 == 31) {
-          tmem_st32(tS + i - 31, pk + i - 31);
-          if (S::kPParts > 1 && i + 1 < S::kPairs) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->p_full[wg][0]);
-          }
+        if (i == 31) tmem_st32(tS, pk);
+      }
+      if constexpr (S::kPairs == 48) tmem_st16(tS + 32, pk + 32);
+      l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      // O rescale (rare), once PV(j-1) has landed: committed with S(j+1) when
+      // that tile exists, else (j = n-1) as the item's first PV-only batch.
+      if (__any_sync(0xffffffffu, need)) {
+        const bool ok = (j + 1 < n) ? warp_wait(&ctl->s_full[wg][(j + 1) & 1], s_parity(j + 1), abort_flag, a.status,
+                                                kSiteODone, a.timeout_ns)
+                                    : warp_wait(&ctl->pv_prev[wg], (base_bits >> 3) & 1, abort_flag, a.status,
+                                                kSiteODone, a.timeout_ns);
+        if (!ok) return;
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < D / 16; ++h) {
+          uint32_t o[16];
+          tmem_ld16(tO + 16 * h, o);
+          tmem_wait_ld_regs<16>(o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(u2f(o[i]) * factor);
+          tmem_st16(tO + 16 * h, o);
         }
       }
-      if constexpr (S::kPairs % 32 == 16) tmem_st16(tS + S::kPairs - 16, pk + S::kPairs - 16);
-      l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-      if (S::kPParts == 1 && any_need && !rescale()) return;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->p_full[wg][S::kPParts - 1 + b]);
+      if (lane == 0) mbar_arrive(&ctl->p_full[wg][b]);
     }
 
     // The next item's hand-off while PV(n-1) runs.
@@ -394,10 +376,7 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
     if (n > 0) {
       if (!warp_wait(&ctl->pv_last[wg], (base_bits >> 2) & 1, abort_flag, a.status, kSiteODone, a.timeout_ns)) return;
       tc_fence_after();
-      if (S::kSBufs == 2)
-        base_bits ^= (((n + 1) >> 1) & 1) | (((n >> 1) & 1) << 1) | 4u | (n > 1 ? 8u : 0u);
-      else
-        base_bits ^= (n & 1) | 4u;
+      base_bits ^= (((n + 1) >> 1) & 1) | (((n >> 1) & 1) << 1) | 4u | (n > 1 ? 8u : 0u);
     }
     const float inv_l = 1.0f / l;
     const bool empty = lim < 0;
@@ -611,27 +590,23 @@ __device__ void producer_role(const Args& a, const CUtensorMap* tm_q, const CUte
     }
     for (uint32_t j = 0; ok && j < it.n; ++j) {
       const int key = it.k_row + static_cast<int>(j) * S::kBN;
-      // K and V of the tile, in one slot or in two.
-#pragma unroll
-      for (int part = 0; part < 3 - S::kSBufs; ++part) {
-        const uint32_t st = g % S::kSlots;
-        if (g >= S::kSlots && !warp_wait(&ctl->kv_empty[st], ((g / S::kSlots) - 1) & 1, abort_flag, a.status,
-                                         kSiteKvEmpty, a.timeout_ns)) {
-          ok = false;
-          break;
-        }
-        if (lead) {
-          uint8_t* slot = sKv + st * S::kSlotBytes;
-          mbar_arrive_expect_tx(&ctl->kv_full[st], S::kSlotBytes);
-#pragma unroll
-          for (int t = 0; t < S::kSBufs; ++t)
-#pragma unroll
-            for (int h = 0; h < S::kHalves; ++h)
-              tma_load_3d(part + t ? tm_v : tm_k, &ctl->kv_full[st], slot + t * S::kKvTileBytes + h * S::kKvHalf,
-                          64 * h, static_cast<int>(it.head), key);
-        }
-        ++g;
+      const uint32_t st = g % S::kSlots;
+      if (g >= S::kSlots && !warp_wait(&ctl->kv_empty[st], ((g / S::kSlots) - 1) & 1, abort_flag, a.status,
+                                       kSiteKvEmpty, a.timeout_ns)) {
+        ok = false;
+        break;
       }
+      if (lead) {
+        uint8_t* slot = sKv + st * S::kSlotBytes;
+        mbar_arrive_expect_tx(&ctl->kv_full[st], S::kSlotBytes);
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h) {
+          tma_load_3d(tm_k, &ctl->kv_full[st], slot + h * S::kKvHalf, 64 * h, static_cast<int>(it.head), key);
+          tma_load_3d(tm_v, &ctl->kv_full[st], slot + S::kKvTileBytes + h * S::kKvHalf, 64 * h,
+                      static_cast<int>(it.head), key);
+        }
+      }
+      ++g;
     }
   }
   // Every copy this warp asked for lands before the CTA can exit.
@@ -659,17 +634,15 @@ __device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sKv, Ctrl<
   // block, then to the next block; a 16-key step of V advances by 2048 B, and
   // V's second block of 64 columns lies a leading-dimension stride on.
   const uint64_t q_desc0 = sdesc_sw128(smem_u32(sQ + wg * S::kQBufs * S::kQTileBytes), 16, 1024);
-  // A slot's K is at its start, its V behind K where the two share a slot.
-  constexpr uint32_t kVOffset = (S::kSBufs - 1) * S::kKvTileBytes;
   const uint64_t k_desc = sdesc_sw128(smem_u32(sKv), 16, 1024);
-  const uint64_t v_desc = sdesc_sw128(smem_u32(sKv) + kVOffset, S::kKvHalf, 1024);
+  const uint64_t v_desc = sdesc_sw128(smem_u32(sKv) + S::kKvTileBytes, S::kKvHalf, 1024);
   constexpr uint64_t kSlotStep = S::kSlotBytes >> 4;
   constexpr uint64_t kQTileStep = S::kQTileBytes >> 4;
   const uint32_t o_tmem = tmem + S::col_o(wg);
   uint32_t p_base0 = 0, p_base1 = 0;  // p_full completions before this item, per buffer
   uint32_t q_used = 0;
-  RingPos<S::kSlots> s_pos;   // next slot to wait for (two score buffers: K and V of a tile)
-  RingPos<S::kSlots> pv_pos;  // two score buffers: next slot whose V feeds a PV product
+  RingPos<S::kSlots> s_pos;   // next slot to wait for (score products, or release)
+  RingPos<S::kSlots> pv_pos;  // next slot whose V feeds a PV product
   bool ok = true;
 
   auto issue_s = [&](uint64_t q_desc, uint32_t st, int buf) {
@@ -680,16 +653,12 @@ __device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sKv, Ctrl<
       umma_ss_elect(d, q_desc + (k >> 2) * (S::kQHalf >> 4) + 2 * (k & 3), kd + (k >> 2) * (S::kKvHalf >> 4) + 2 * (k & 3),
                     idesc_qk, k > 0 ? 1u : 0u);
   };
-  // Part `part` of the tile's PV product (of kPParts).
-  auto issue_pv = [&](uint32_t st, int buf, int part, bool acc) {
+  auto issue_pv = [&](uint32_t st, int buf, bool acc) {
     const uint64_t vd = v_desc + st * kSlotStep;
     const uint32_t p = tmem + S::col_s(wg, buf);
-    constexpr int kSteps = kBN / 16 / S::kPParts;
 #pragma unroll
-    for (int x = 0; x < kSteps; ++x) {
-      const int k = part * kSteps + x;
+    for (int k = 0; k < kBN / 16; ++k)
       umma_ts_elect(o_tmem, p + 8 * k, vd + 128 * k, idesc_pv, (acc || k > 0) ? 1u : 0u);
-    }
   };
   auto kv_wait = [&](const RingPos<S::kSlots>& r) {
     return warp_wait(&ctl->kv_full[r.slot], r.phase, abort_flag, a.status, kSiteKvFull, a.timeout_ns);
@@ -697,7 +666,7 @@ __device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sKv, Ctrl<
   // Values behind the sequence's end become zero.  Both MMA warps write the
   // same zeros; a warp's own products are issued behind its fence.
   auto clear_tail = [&](uint32_t st, int keys) {
-    uint8_t* v = sKv + st * S::kSlotBytes + kVOffset;
+    uint8_t* v = sKv + st * S::kSlotBytes + S::kKvTileBytes;
     const int lane = threadIdx.x & 31;
     for (int x = keys * 8 + lane; x < kBN * 8; x += 32) {
 #pragma unroll
@@ -735,103 +704,58 @@ __device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sKv, Ctrl<
       const uint64_t q_desc = q_desc0 + qb * kQTileStep;
       // Keys of this warpgroup's last tile that belong to the sequence, if not all do.
       const int tail = it.n_keys - static_cast<int>(n - 1) * kBN;
-      if constexpr (S::kSBufs == 2) {
-        // S(0) and S(1) up front.  The commit after the item's last S also frees its Q buffer.
-        for (uint32_t t = 0; t < 2 && t < n; ++t) {
-          if (!kv_wait(s_pos)) {
-            ok = false;
-            break;
-          }
-          issue_s(q_desc, s_pos.slot, static_cast<int>(t));
-          s_pos.next();
-          umma_commit_elect(&ctl->s_full[wg][t]);
-          if (t == n - 1) {
-            umma_commit_elect(&ctl->q_empty[wg][qb]);
-            if (!fetch_next(k + 1)) ok = false;
-          }
+      // S(0) and S(1) up front.  The commit after the item's last S also frees its Q buffer.
+      for (uint32_t t = 0; t < 2 && t < n; ++t) {
+        if (!kv_wait(s_pos)) {
+          ok = false;
+          break;
         }
-        for (uint32_t j = 0; ok && j < n; ++j) {
-          const int b = static_cast<int>(j & 1);
-          const uint32_t st = pv_pos.slot;  // V_j: waited on before S(j) was issued
-          pv_pos.next();
-          if (j + 1 == n && tail < kBN) clear_tail(st, tail);
-          if (!warp_wait(&ctl->p_full[wg][b], ((b ? p_base1 : p_base0) + (j >> 1)) & 1, abort_flag, a.status,
-                         kSitePFull, a.timeout_ns)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          issue_pv(st, b, 0, j > 0);
-          if (j + 2 < n) {
-            if (!kv_wait(s_pos)) {
-              ok = false;
-              break;
-            }
-            issue_s(q_desc, s_pos.slot, b);  // after PV(j) in this warp's order: P(j) is read first
-            s_pos.next();
-            umma_commit_elect(&ctl->s_full[wg][b]);
-            if (j + 2 == n - 1) {
-              umma_commit_elect(&ctl->q_empty[wg][qb]);
-              if (!fetch_next(k + 1)) {
-                ok = false;
-                break;
-              }
-            }
-          } else {
-            umma_commit_elect(j + 1 == n ? &ctl->pv_last[wg] : &ctl->pv_prev[wg]);
-          }
-          umma_commit_elect(&ctl->kv_empty[st]);
-        }
-      } else {
-        // S(0); then per tile PV(j) part by part and S(j+1), which overwrites P(j)
-        // behind it.  Slots: K(j), V(j), K(j+1), ...; S(j) frees K(j), PV(j) V(j).
-        for (uint32_t j = 0; ok && j <= n; ++j) {
-          if (j > 0) {  // PV(j-1)
-            const uint32_t t = j - 1;
-            if (!kv_wait(s_pos)) {
-              ok = false;
-              break;
-            }
-            const uint32_t st = s_pos.slot;
-            s_pos.next();
-            if (t + 1 == n && tail < kBN) clear_tail(st, tail);
-  #pragma unroll
-            for (int part = 0; part < S::kPParts; ++part) {
-              if (!warp_wait(&ctl->p_full[wg][part], (p_base0 + t) & 1, abort_flag, a.status, kSitePFull,
-                             a.timeout_ns)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              issue_pv(st, 0, part, t > 0);
-            }
-            if (!ok) break;
-            umma_commit_elect(&ctl->kv_empty[st]);
-          }
-          if (j == n) {
-            umma_commit_elect(&ctl->pv_last[wg]);
-            break;
-          }
-          if (!kv_wait(s_pos)) {
-            ok = false;
-            break;
-          }
-          issue_s(q_desc, s_pos.slot, 0);
-          umma_commit_elect(&ctl->s_full[wg][0]);
-          umma_commit_elect(&ctl->kv_empty[s_pos.slot]);
-          s_pos.next();
-          if (j == n - 1) {
-            umma_commit_elect(&ctl->q_empty[wg][qb]);
-            if (!fetch_next(k + 1)) ok = false;
-          }
+        issue_s(q_desc, s_pos.slot, static_cast<int>(t));
+        s_pos.next();
+        umma_commit_elect(&ctl->s_full[wg][t]);
+        if (t == n - 1) {
+          umma_commit_elect(&ctl->q_empty[wg][qb]);
+          if (!fetch_next(k + 1)) ok = false;
         }
       }
-      p_base0 += S::kSBufs == 2 ? (n + 1) >> 1 : n;
+      for (uint32_t j = 0; ok && j < n; ++j) {
+        const int b = static_cast<int>(j & 1);
+        const uint32_t st = pv_pos.slot;  // V_j: waited on before S(j) was issued
+        pv_pos.next();
+        if (j + 1 == n && tail < kBN) clear_tail(st, tail);
+        if (!warp_wait(&ctl->p_full[wg][b], ((b ? p_base1 : p_base0) + (j >> 1)) & 1, abort_flag, a.status,
+                       kSitePFull, a.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        issue_pv(st, b, j > 0);
+        if (j + 2 < n) {
+          if (!kv_wait(s_pos)) {
+            ok = false;
+            break;
+          }
+          issue_s(q_desc, s_pos.slot, b);  // after PV(j) in this warp's order: P(j) is read first
+          s_pos.next();
+          umma_commit_elect(&ctl->s_full[wg][b]);
+          if (j + 2 == n - 1) {
+            umma_commit_elect(&ctl->q_empty[wg][qb]);
+            if (!fetch_next(k + 1)) {
+              ok = false;
+              break;
+            }
+          }
+        } else {
+          umma_commit_elect(j + 1 == n ? &ctl->pv_last[wg] : &ctl->pv_prev[wg]);
+        }
+        umma_commit_elect(&ctl->kv_empty[st]);
+      }
+      p_base0 += (n + 1) >> 1;
       p_base1 += n >> 1;
       ++q_used;
     }
     // Tiles only the other warpgroup needs: released once they have landed.
-    for (uint32_t j = n * (3 - S::kSBufs); ok && j < it.n * (3 - S::kSBufs); ++j, s_pos.next()) {
+    for (uint32_t j = n; ok && j < it.n; ++j, s_pos.next()) {
       if (!kv_wait(s_pos)) {
         ok = false;
         break;

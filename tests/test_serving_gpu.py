@@ -5,8 +5,8 @@ attention_paged (one token per sequence), alone and as a prompt followed by sing
 Tolerances, per element, from the operators' arithmetic.  u = eps / 2 of the storage type.
 - A rotated element is two f32 products and a sum rounded once: u |y| + 2^-22 (|x c| + |x' s|),
   and half the smallest f16 subnormal, 2^-25.
-- An attention output is sum w_j v_j / sum w_j with weights rounded to the storage type before
-  both sums (relative u each), exponentials good to 1e-4 (cubic of the FMA pipe: 8.3e-5) and
+- An attention output is sum w_j v_j / sum w_j with weights rounded to the storage type in the
+  first sum, or in both (relative u each), exponentials good to 1e-4 (cubic of the FMA pipe: 8.3e-5) and
   exponents s c wrong by at most |s c| 2^-22 + D 2^-23 sum_e |q_e k_e| c, which max |s| <= 64 keeps
   below 2^-9 for the inputs here (|q.k| scale <= 16 with unit normals).  A weight's relative
   error e moves the output by at most e sum w_j |v_j - o| / sum w_j <= 2 e A with A = sum w_j |v_j|
@@ -18,7 +18,7 @@ import math
 import pytest
 import torch
 
-from headshot_b200._lib import HS_ERR_INVALID, HsError
+from headshot_b200._lib import HS_ERR_INVALID, HS_ERR_TIMEOUT, HsError
 from headshot_b200.engine import GpuContext, PagedKv, Rope
 
 pytestmark = pytest.mark.gpu
@@ -318,6 +318,27 @@ def test_varlen_bad_offsets_are_reported(gpu_ctx):
     again = gpu_ctx.attention_varlen(q, k, v, offsets([20, 20]))
     gpu_ctx.sync()
     assert torch.equal(good, again)
+
+
+def test_varlen_timeout_is_reported_and_leaves_the_context_usable():
+    """Wait bound 0: every in-kernel wait that has to wait gives up at once (no fault, no hang)."""
+    ctx = GpuContext(0)
+    g = gen(13)
+    lens = [900, 300]
+    for d in (64, 128):
+        q, k, v = (normal(g, 1200, h, d) for h in (8, 2, 2))
+        good = ctx.attention_varlen(q, k, v, offsets(lens))
+        ctx.sync()
+        ctx.set_wait_timeout_ms(0)
+        ctx.attention_varlen(q, k, v, offsets(lens))
+        with pytest.raises(HsError) as e:
+            ctx.sync()
+        assert e.value.status == HS_ERR_TIMEOUT
+        ctx.set_wait_timeout_ms(2000)
+        again = ctx.attention_varlen(q, k, v, offsets(lens))
+        ctx.sync()
+        assert torch.equal(good, again)
+    ctx.close()
 
 
 # ---------------------------------------------------------- attention_paged --
