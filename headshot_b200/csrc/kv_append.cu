@@ -14,8 +14,10 @@
 // partners [D/2 + 8c, +8).  It loads the chunk's 32 table values once and then
 // takes every lane-th head of the token with them, kBatch heads' loads in
 // flight before the first store, so a head row costs two 16-byte loads and
-// two 16-byte stores and the table stays out of the loop.  An element is read
-// and written by the same thread, so q_out may be q and k_out may be k.
+// two 16-byte stores and the table stays out of the loop.  The first heads'
+// loads are issued before the token's place (sequence, length, page, table row)
+// is looked up, so the four dependent reads hide behind them.  An element is
+// read and written by the same thread, so q_out may be q and k_out may be k.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -65,6 +67,26 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   const uint32_t in_token = threadIdx.x % per_token;
   const uint32_t chunk = in_token % kChunks;
   const uint32_t lane = in_token / kChunks;
+
+  const uint32_t q_rows = a.q ? a.q_heads : 0;
+  const uint32_t rows = q_rows + 2 * c.heads;
+  const E* qt = static_cast<const E*>(a.q) + token * a.q_stride;
+  const E* kt = static_cast<const E*>(a.k) + token * a.k_stride;
+  const E* vt = static_cast<const E*>(a.v) + token * a.v_stride;
+  uint4 lo[kBatch], hi[kBatch];
+  auto load = [&](uint32_t r0) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const uint32_t r = r0 + b * lanes;
+      if (r >= rows) break;
+      const E* src = r < q_rows             ? qt + static_cast<uint64_t>(r) * D
+                     : r < q_rows + c.heads ? kt + static_cast<uint64_t>(r - q_rows) * D
+                                            : vt + static_cast<uint64_t>(r - q_rows - c.heads) * D;
+      lo[b] = *reinterpret_cast<const uint4*>(src + 8 * chunk);
+      hi[b] = *reinterpret_cast<const uint4*>(src + D / 2 + 8 * chunk);
+    }
+  };
+  load(lane);  // in flight while the token's place is looked up: four dependent reads
 
   uint32_t seq = token;
   int64_t pos;
@@ -119,23 +141,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     }
   }
 
-  const uint32_t q_rows = a.q ? a.q_heads : 0;
-  const uint32_t rows = q_rows + 2 * c.heads;
-  const E* qt = static_cast<const E*>(a.q) + token * a.q_stride;
-  const E* kt = static_cast<const E*>(a.k) + token * a.k_stride;
-  const E* vt = static_cast<const E*>(a.v) + token * a.v_stride;
-  for (uint32_t r0 = lane; r0 < rows; r0 += kBatch * lanes) {
-    uint4 lo[kBatch], hi[kBatch];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const uint32_t r = r0 + b * lanes;
-      if (r >= rows) break;
-      const E* src = r < q_rows                ? qt + static_cast<uint64_t>(r) * D
-                     : r < q_rows + c.heads ? kt + static_cast<uint64_t>(r - q_rows) * D
-                                            : vt + static_cast<uint64_t>(r - q_rows - c.heads) * D;
-      lo[b] = *reinterpret_cast<const uint4*>(src + 8 * chunk);
-      hi[b] = *reinterpret_cast<const uint4*>(src + D / 2 + 8 * chunk);
-    }
+  for (uint32_t r0 = lane; r0 < rows;) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const uint32_t r = r0 + b * lanes;
@@ -166,6 +172,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
         if (!is_v && a.k_out) put(static_cast<E*>(a.k_out) + (static_cast<uint64_t>(token) * c.heads + h) * D);
       }
     }
+    r0 += kBatch * lanes;
+    load(r0);
   }
 }
 

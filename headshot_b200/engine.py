@@ -261,7 +261,7 @@ class GpuContext:
             assert nq == n and dq == d and q.dtype is dtype, "q tokens, head_dim or dtype mismatch"
             assert hq % hkv == 0, "q heads must be a multiple of k heads"
             if q_out is None:
-                q_out = torch.empty((n, hq, d), dtype=dtype, device=q.device)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             else:
                 self._check_out(q_out, q, "q_out")
         else:
@@ -307,7 +307,7 @@ class GpuContext:
         else:
             assert tk == t, "without cu_k, k and v have as many tokens as q"
         if out is None:
-            out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             self._check_out(out, q, "out")
         if out.numel() == 0:
@@ -336,7 +336,7 @@ class GpuContext:
         assert cd == d, "q head_dim"
         assert hkv > 0 and hq % hkv == 0, "q heads must be a multiple of k heads"
         if out is None:
-            out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             self._check_out(out, q, "out")
         if out.numel() == 0:
