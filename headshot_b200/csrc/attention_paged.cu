@@ -7,7 +7,7 @@
 // read once (4 Hkv D bytes per key) for 4 Hq D flops per key, so HBM bounds
 // it; a single short sequence is bound by latency.
 //
-// Work is cut in tiles of 64 keys of one (sequence, key head, head tile)
+// Work is cut in tiles of 64 or 128 keys of one (sequence, key head, head tile)
 // item, numbered through all items (an item has kItemCost numbers more than
 // tiles, for its end).  The grid is fixed; each CTA finds the
 // total from the lengths on the device and takes an equal contiguous range of
@@ -19,19 +19,26 @@
 // returns the counter to zero.  A CTA cuts at most its first and its last
 // item: two partials and one counter each, whatever the shape.
 //
-// Inside a CTA, warp w takes keys [16w, 16w + 16) of every tile through a
+// Inside a CTA, each warp takes a quarter of every tile's keys through a
 // ring of its own (cp.async, kStages deep, running on across items): no block
 // barrier until an item ends, when the four warps' states are joined through
 // the ring stage just consumed.  Scores and values go through mma.sync
 // m16n8k16 with the 16 rows holding query heads: at 4 heads per key three
-// quarters of the tensor work is padding, but HBM delivers a warp's 16 keys
-// more slowly than the padded products take (tcgen05's 128-row tile would
+// quarters of the tensor work is padding, but HBM delivers a warp's keys more
+// slowly than the padded products take (tcgen05's 128-row tile would
 // pad 32-fold).  Rows are stored with 16-byte chunks XORed by the row's low
 // bits, which makes ldmatrix free of bank conflicts.  Weights are rounded to
 // the storage type for the second product, and the sum adds the rounded
 // weights, so the rounding of dominant weights cancels; statistics and
-// accumulators are f32.  Keys past the length are never read (the ring is
-// zero-filled there).
+// accumulators are f32.  (Weights split in two 16-bit parts, so that nothing is
+// rounded away, cost 5 % at head_dim 64.)  Keys past the length are never read
+// (the ring is zero-filled there).
+//
+// Measured: 128 sequences of 1 to 16,001 keys, 32/8 x 128: 166 us, 6.5 TB/s;
+// 274,800 keys, 16 x 64: 170 us, 6.6 TB/s (a plain copy reaches 6.55).  One
+// sequence of 8,191 keys, 32/8 x 128: 15.6 us for 5.1 us of reading: launch 1.1,
+// range 1.2, keys and values 8.3, join of the warps 0.9, partials written and
+// counted 1.0, 33 of them joined 3.2.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -44,28 +51,34 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kWarpKeys = 16;
-constexpr int kTileKeys = kWarps * kWarpKeys;
 constexpr int kRows = 16;  // query heads per item
 constexpr uint32_t kMaxCtas = 1024;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: weights stay below 2^8 between rescales
 
+// 8 KB of K and V per warp and tile either way.  Head_dim 128: three stages and
+// two CTAs per SM (255 registers; three CTAs of two stages spill, 1.9 times
+// slower).  Head_dim 64 (200 x 1,374 keys, 16 x 64): 170 us like this, 173 us
+// with three stages and two CTAs, 182 us with 16 keys per warp, four stages
+// and three CTAs.
 template <int D>
 struct Shape {
-  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kWarpKeys = D == 128 ? 16 : 32;
+  static constexpr int kTileKeys = kWarps * kWarpKeys;
+  static constexpr int kStages = D == 128 ? 3 : 2;
   static constexpr int kCtasPerSm = D == 128 ? 2 : 3;
-  static constexpr int kStageBytes = kWarpKeys * D * 2 * 2;  // K rows, then V rows; also 16 x D f32
+  static constexpr int kStageBytes = kWarpKeys * D * 2 * 2;  // K rows, then V rows; holds 16 x D f32 too
   static constexpr int kSmem = kWarps * kStages * kStageBytes;
+  // An item's end costs a CTA about as much as 128 keys (query loads, the join
+  // of the warps), so each item takes that many numbers more than its tiles:
+  // 128 sequences of 1 to 16,001 keys, 32/8 x 128, 219 us without them, 168 us
+  // with 64, 128 or 256 keys' worth.
+  static constexpr uint32_t kItemCost = 128 / kTileKeys;
+  // Fewest numbers per CTA.  With 128 keys' worth, 64 sequences of 100 keys
+  // take 13.6 us instead of 12.6, because items that fit one CTA are cut; with
+  // 512, 17.0 us.
+  static constexpr uint32_t kMinTiles = 256 / kTileKeys;
 };
-
-// An item's end costs a CTA about as much as two tiles (query loads, the join
-// of the warps), so each item takes two numbers more than its tiles: 128
-// sequences of 1 to 16,001 keys, 219 us without them, 165 us with 1, 2 or 4.
-constexpr uint32_t kItemCost = 2;
-// Fewest numbers per CTA: with 2, 64 sequences of 100 keys (two tiles an
-// item) take 13.6 us instead of 12.6, because items that fit one CTA are cut;
-// with 8, 17.0 us.
-constexpr uint32_t kMinTiles = 4;
+constexpr int kMaxCtasPerSm = 3;
 
 // Workspace: counters, then per CTA two partials of (16 x 128 O, 16 m, 16 l) f32.
 constexpr size_t kCounterBytes = kMaxCtas * sizeof(uint32_t);
@@ -127,7 +140,10 @@ __device__ __forceinline__ uint32_t seq_len(const Args& a, uint32_t s) {
   return static_cast<uint32_t>(n);
 }
 // An empty sequence has one tile too, which writes its zeros.
-__device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return len ? (len + kTileKeys - 1) / kTileKeys : 1; }
+template <int D>
+__device__ __forceinline__ uint32_t tiles_of(uint32_t len) {
+  return len ? (len + Shape<D>::kTileKeys - 1) / Shape<D>::kTileKeys : 1;
+}
 
 // A place in the numbering of tiles: tile `tile` of item (seq, sub).
 struct Place {
@@ -135,16 +151,17 @@ struct Place {
   uint32_t seq, sub, tile, tiles, len;
 };
 
+template <int D>
 __device__ __forceinline__ void next_tile(const Args& a, Place& p) {
   ++p.at;
   if (++p.tile < p.tiles) return;
-  p.at += kItemCost;
+  p.at += Shape<D>::kItemCost;
   p.tile = 0;
   if (++p.sub < a.subs) return;
   p.sub = 0;
   if (++p.seq < a.c.n_seqs) {
     p.len = seq_len(a, p.seq);
-    p.tiles = tiles_of(p.len);
+    p.tiles = tiles_of<D>(p.len);
   }
 }
 
@@ -179,12 +196,13 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, S
   return total;
 }
 
-// Issues this warp's 16 keys of a tile into its ring stage.
+// Issues this warp's keys of a tile into its ring stage.
 template <typename E, int D, bool kWholeSteps>
 __device__ __forceinline__ void load_tile(const Args& a, const Place& p, uint32_t stage, int warp, int lane) {
+  using S = Shape<D>;
   constexpr int kChunks = D / 8;            // 16-byte chunks per row
   constexpr int kRowsPer = 32 / kChunks;    // rows one warp instruction covers
-  const uint32_t key0 = p.tile * kTileKeys + warp * kWarpKeys;
+  const uint32_t key0 = p.tile * S::kTileKeys + warp * S::kWarpKeys;
   if (key0 >= p.len) return;
   const uint32_t chunk = lane % kChunks;
   const uint32_t head = p.sub / a.head_tiles;
@@ -203,27 +221,30 @@ __device__ __forceinline__ void load_tile(const Args& a, const Place& p, uint32_
     }
     return (static_cast<uint64_t>(page) * a.c.heads + head) * a.c.page_size;
   };
-  bool page_ok = true;
-  uint32_t off0 = 0;
-  uint64_t row0 = 0;
-  if (kWholeSteps) row0 = page_row(key0, &off0, &page_ok);  // 16 keys never straddle pages
 #pragma unroll
-  for (int i = 0; i < kWarpKeys / kRowsPer; ++i) {
-    const uint32_t r = i * kRowsPer + lane / kChunks;
-    bool ok = key0 + r < p.len;
-    uint64_t at;
-    if (kWholeSteps) {
-      ok = ok && page_ok;
-      at = (row0 + off0 + r) * D;
-    } else {
-      uint32_t off = 0;
-      at = ok ? page_row(key0 + r, &off, &ok) : 0;
-      at = (at + off) * D;
+  for (int step = 0; step < S::kWarpKeys; step += 16) {
+    bool page_ok = key0 + step < p.len;
+    uint32_t off0 = 0;
+    uint64_t row0 = 0;
+    if (kWholeSteps && page_ok) row0 = page_row(key0 + step, &off0, &page_ok);  // 16 keys never straddle pages
+#pragma unroll
+    for (int i = 0; i < 16 / kRowsPer; ++i) {
+      const uint32_t r = step + i * kRowsPer + lane / kChunks;
+      bool ok = key0 + r < p.len;
+      uint64_t at;
+      if (kWholeSteps) {
+        ok = ok && page_ok;
+        at = (row0 + off0 + r - step) * D;
+      } else {
+        uint32_t off = 0;
+        at = ok ? page_row(key0 + r, &off, &ok) : 0;
+        at = (at + off) * D;
+      }
+      if (!ok) at = 0;
+      const uint32_t dst = stage + r * (D * 2) + ((chunk ^ (r & 7)) << 4);
+      cp_async16(dst, kc + at, ok);
+      cp_async16(dst + S::kWarpKeys * D * 2, vc + at, ok);
     }
-    if (!ok) at = 0;
-    const uint32_t dst = stage + r * (D * 2) + ((chunk ^ (r & 7)) << 4);
-    cp_async16(dst, kc + at, ok);
-    cp_async16(dst + kWarpKeys * D * 2, vc + at, ok);
   }
 }
 
@@ -236,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
 
   // The CTA's range of numbers, and the sequence it starts in.  `first` and
   // `n` are this thread's sequence of the chunk scanned last.
-  auto numbers = [&](uint32_t s) -> uint32_t { return s < a.c.n_seqs ? tiles_of(seq_len(a, s)) + kItemCost : 0u; };
+  auto numbers = [&](uint32_t s) -> uint32_t { return s < a.c.n_seqs ? tiles_of<D>(seq_len(a, s)) + S::kItemCost : 0u; };
   uint32_t n = numbers(tid);
   unsigned long long first;
   unsigned long long chunk = block_scan(n, &sh, &first);
@@ -249,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
   }
   total *= a.subs;
   const unsigned long long even = (total + gridDim.x - 1) / gridDim.x;
-  const unsigned long long per = even < kMinTiles ? kMinTiles : even;
+  const unsigned long long per = even < S::kMinTiles ? S::kMinTiles : even;
   const unsigned long long start = blockIdx.x * per;
   if (start >= total) return;
   const unsigned long long end = start + per < total ? start + per : total;
@@ -271,14 +292,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
   Place cur;
   cur.seq = sh.start_seq;
   cur.len = seq_len(a, cur.seq);
-  cur.tiles = tiles_of(cur.len);
-  cur.sub = static_cast<uint32_t>(sh.start_off / (cur.tiles + kItemCost));
-  cur.tile = static_cast<uint32_t>(sh.start_off % (cur.tiles + kItemCost));
+  cur.tiles = tiles_of<D>(cur.len);
+  cur.sub = static_cast<uint32_t>(sh.start_off / (cur.tiles + S::kItemCost));
+  cur.tile = static_cast<uint32_t>(sh.start_off % (cur.tiles + S::kItemCost));
   cur.at = start;
   if (cur.tile >= cur.tiles) {  // starts among an item's extra numbers: on to the next item
     cur.at -= cur.tile - (cur.tiles - 1);
     cur.tile = cur.tiles - 1;
-    next_tile(a, cur);
+    next_tile<D>(a, cur);
   }
 
   const uint32_t my_ring = smem_u32(ring) + warp * S::kStages * S::kStageBytes;
@@ -287,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
   auto load_next = [&] {
     if (ahead.at < end) {
       load_tile<E, D, kWholeSteps>(a, ahead, my_ring + load_stage * S::kStageBytes, warp, lane);
-      next_tile(a, ahead);
+      next_tile<D>(a, ahead);
     }
     load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
     cp_async_commit();
@@ -327,22 +348,25 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
     __syncwarp();
     load_next();
     const uint32_t stage = my_ring + st * S::kStageBytes;
-    const uint32_t key0 = cur.tile * kTileKeys + warp * kWarpKeys;
+    const uint32_t key0 = cur.tile * S::kTileKeys + warp * S::kWarpKeys;
     if (key0 < cur.len) {
-      // Scores: rows = heads, two 8-key column tiles.
-      float s[2][4] = {};
+      // Scores: rows = heads, 8-key column tiles.
+      constexpr int kCols = S::kWarpKeys / 8;
+      float s[kCols][4] = {};
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        uint32_t b[4];
-        const uint32_t r = (lane & 7) + ((lane >> 4) << 3), ch = 2 * k + ((lane >> 3) & 1);
-        ldsm4(b, stage + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-        mma16816<E>(s[0], q[k], b[0], b[1]);
-        mma16816<E>(s[1], q[k], b[2], b[3]);
-      }
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int t = 0; t < kCols; t += 2) {
+          uint32_t b[4];
+          const uint32_t r = 8 * t + (lane & 7) + ((lane >> 4) << 3), ch = 2 * k + ((lane >> 3) & 1);
+          ldsm4(b, stage + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+          mma16816<E>(s[t], q[k], b[0], b[1]);
+          mma16816<E>(s[t + 1], q[k], b[2], b[3]);
+        }
       const uint32_t valid = cur.len - key0;
-      if (valid < kWarpKeys) {
+      if (valid < S::kWarpKeys) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < kCols; ++t)
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             if (t * 8 + 2 * (lane & 3) + (x & 1) >= valid) s[t][x] = -INFINITY;
@@ -350,7 +374,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
       float top[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float t = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+        float t = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+#pragma unroll
+        for (int x = 1; x < kCols; ++x) t = fmaxf(t, fmaxf(s[x][2 * h], s[x][2 * h + 1]));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
         top[h] = t * a.scale_log2;
@@ -369,26 +395,28 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
           }
         }
       }
-      uint32_t p[4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int g = 0; g < kCols; g += 2) {  // 16 keys
+        uint32_t p[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float base_m = m[h] == -INFINITY ? 0.f : m[h];
-          const float e0 = ex2_approx(fmaf(s[t][2 * h], a.scale_log2, -base_m));
-          const float e1 = ex2_approx(fmaf(s[t][2 * h + 1], a.scale_log2, -base_m));
-          const uint32_t w = Elem<E>::pack2(e0, e1);
-          p[2 * t + h] = w;
-          const float2 f = Elem<E>::unpack2(w);
-          l[h] += f.x + f.y;
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float base_m = m[h] == -INFINITY ? 0.f : m[h];
+            const uint32_t w = Elem<E>::pack2(ex2_approx(fmaf(s[g + t][2 * h], a.scale_log2, -base_m)),
+                                              ex2_approx(fmaf(s[g + t][2 * h + 1], a.scale_log2, -base_m)));
+            const float2 f = Elem<E>::unpack2(w);
+            l[h] += f.x + f.y;
+            p[2 * t + h] = w;
+          }
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          uint32_t b[4];
+          const uint32_t r = 8 * g + (lane & 7) + (((lane >> 3) & 1) << 3), ch = 2 * n + (lane >> 4);
+          ldsm4_t(b, stage + S::kWarpKeys * D * 2 + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+          mma16816<E>(o[2 * n], p, b[0], b[1]);
+          mma16816<E>(o[2 * n + 1], p, b[2], b[3]);
         }
-#pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        uint32_t b[4];
-        const uint32_t r = (lane & 7) + (((lane >> 3) & 1) << 3), ch = 2 * n + (lane >> 4);
-        ldsm4_t(b, stage + kWarpKeys * D * 2 + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-        mma16816<E>(o[2 * n], p, b[0], b[1]);
-        mma16816<E>(o[2 * n + 1], p, b[2], b[3]);
       }
     }
 
@@ -511,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
       __syncthreads();  // the stage and sh may be written again
       fresh = true;
     }
-    next_tile(a, cur);
+    next_tile<D>(a, cur);
   }
   cp_async_wait<0>();
 }
@@ -525,23 +553,23 @@ cudaError_t launch(cudaStream_t stream, const Args& a) {
   uint64_t ctas = static_cast<uint64_t>(current_sm_count()) * S::kCtasPerSm;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   // No more CTAs than the block table has work for.
-  const uint64_t most = (static_cast<uint64_t>(a.c.max_pages) * a.c.page_size + kTileKeys - 1) / kTileKeys;
+  const uint64_t most = (static_cast<uint64_t>(a.c.max_pages) * a.c.page_size + S::kTileKeys - 1) / S::kTileKeys;
   const uint64_t tiles = static_cast<uint64_t>(a.c.n_seqs) * a.subs * (most ? most : 1);
-  if (ctas > (tiles + kMinTiles - 1) / kMinTiles) ctas = (tiles + kMinTiles - 1) / kMinTiles;
+  if (ctas > (tiles + S::kMinTiles - 1) / S::kMinTiles) ctas = (tiles + S::kMinTiles - 1) / S::kMinTiles;
   attention_paged_kernel<E, D, kWholeSteps><<<static_cast<uint32_t>(ctas), kThreads, S::kSmem, stream>>>(a);
   return cudaGetLastError();
 }
 
 template <typename E, int D>
 cudaError_t launch_pages(cudaStream_t stream, const Args& a) {
-  // Pages of a multiple of 16 keys: one table entry serves a warp's 16 keys.
-  return a.c.page_size % kWarpKeys == 0 ? launch<E, D, true>(stream, a) : launch<E, D, false>(stream, a);
+  // Pages of a multiple of 16 keys: one table entry serves 16 keys.
+  return a.c.page_size % 16 == 0 ? launch<E, D, true>(stream, a) : launch<E, D, false>(stream, a);
 }
 
 }  // namespace
 
 size_t attention_paged_workspace_bytes() {
-  uint64_t ctas = static_cast<uint64_t>(current_sm_count()) * Shape<64>::kCtasPerSm;
+  uint64_t ctas = static_cast<uint64_t>(current_sm_count()) * kMaxCtasPerSm;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   return kCounterBytes + ctas * 2 * kPartialFloats * sizeof(float);
 }
