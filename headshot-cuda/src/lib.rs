@@ -276,6 +276,186 @@ impl Context {
     }
 }
 
+/// Device array of i32 indices (lengths, offsets, block tables) for the serving ops.
+pub struct Indices {
+    ptr: *mut c_void,
+    ctx: Context,
+    len: usize,
+}
+
+// SAFETY: as CudaTensor.
+unsafe impl Send for Indices {}
+unsafe impl Sync for Indices {}
+
+impl Indices {
+    pub fn len(&self) -> usize {
+        self.len
+    }
+
+    pub fn is_empty(&self) -> bool {
+        self.len == 0
+    }
+
+    /// Overwrites the array, in stream order (a new step's lengths).
+    pub fn set(&self, values: &[i32]) -> Result<(), Error> {
+        assert_eq!(values.len(), self.len, "index count");
+        let g = self.ctx.lock();
+        check(unsafe { ffi::hs_memcpy_h2d(g.0, self.ptr, values.as_ptr().cast(), 4 * values.len()) })
+    }
+
+    fn ptr(&self) -> *const c_int {
+        self.ptr as *const c_int
+    }
+}
+
+impl Drop for Indices {
+    fn drop(&mut self) {
+        let g = self.ctx.lock();
+        // SAFETY: stream-ordered free, after the work already queued that uses the array.
+        unsafe { ffi::hs_free(g.0, self.ptr) };
+    }
+}
+
+/// A paged key-value cache: k, v (pages, heads, page_size, D) and the (n_seqs, max_pages) block
+/// table; token p of sequence s is row p % page_size of page table[s * max_pages + p / page_size].
+pub struct PagedKv {
+    pub k: CudaTensor,
+    pub v: CudaTensor,
+    pub block_table: Indices,
+    pub n_seqs: usize,
+}
+
+impl PagedKv {
+    /// (pages, heads, page_size, D, max_pages), asserted.
+    fn dims(&self, lens: &Indices) -> (u32, u32, u32, u32, u32) {
+        let [pages, heads, page, d] = self.k.shape[..] else { panic!("cache wants (pages,heads,page_size,D)") };
+        assert_eq!(self.k.shape, self.v.shape);
+        assert!(self.k.dtype == self.v.dtype, "cache: mixed dtypes");
+        assert!(self.n_seqs > 0 && self.block_table.len() % self.n_seqs == 0, "block_table wants (n_seqs, max_pages)");
+        assert_eq!(lens.len(), self.n_seqs, "kv_lens wants one length per sequence");
+        let max_pages = self.block_table.len() / self.n_seqs;
+        (pages as u32, heads as u32, page as u32, d as u32, max_pages as u32)
+    }
+}
+
+/// Serving over a growing token stream (no counterpart in the reference).
+impl Context {
+    pub fn indices(&self, values: &[i32]) -> Result<Indices, Error> {
+        let mut p: *mut c_void = ptr::null_mut();
+        {
+            let g = self.lock();
+            check(unsafe { ffi::hs_alloc(g.0, (4 * values.len()).max(4), &mut p) })?;
+        }
+        let out = Indices { ptr: p, ctx: self.clone(), len: values.len() };
+        out.set(values)?;
+        Ok(out)
+    }
+
+    /// New tokens' k, v (tokens, heads, D) into the cache, k and q rotated on the way; the last new
+    /// token of sequence s takes position kv_lens[s] - 1.  `cu_new` (n_seqs + 1): the sequences'
+    /// tokens; None: one each.  q and q_out go together; k_out receives the rotated keys once more.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_append(&self, cache: &PagedKv, k: &CudaTensor, v: &CudaTensor, kv_lens: &Indices,
+                     cu_new: Option<&Indices>, rope: Option<&Rope<'_>>, q: Option<(&CudaTensor, &CudaTensor)>,
+                     k_out: Option<&CudaTensor>) {
+        let [n, heads, dim] = k.shape[..] else { panic!("kv_append wants k (tokens,heads,D)") };
+        let (pages, hkv, page, d, max_pages) = cache.dims(kv_lens);
+        assert_eq!(k.shape, v.shape);
+        assert!(heads as u32 == hkv && dim as u32 == d, "cache heads and head_dim");
+        assert!(k.dtype == v.dtype && k.dtype == cache.k.dtype, "kv_append: mixed dtypes");
+        match cu_new {
+            Some(c) => assert_eq!(c.len(), cache.n_seqs + 1, "cu_new wants n_seqs + 1 offsets"),
+            None => assert_eq!(n, cache.n_seqs, "without cu_new there is one token per sequence"),
+        }
+        let (q_ptr, q_out, hq) = match q {
+            Some((x, y)) => {
+                let [nq, hq, dq] = x.shape[..] else { panic!("kv_append wants q (tokens,heads,D)") };
+                assert!(nq == n && dq == dim && x.shape == y.shape && x.dtype == k.dtype && y.dtype == k.dtype);
+                (x.ptr as *const c_void, y.ptr, hq as u32)
+            }
+            None => (ptr::null(), ptr::null_mut(), 0),
+        };
+        let k_rot = k_out.map_or(ptr::null_mut(), |t| {
+            assert!(t.shape == k.shape && t.dtype == k.dtype, "k_out shape");
+            t.ptr
+        });
+        let (sin, cos, rows, prefix, tpf) = match rope {
+            Some(r) => {
+                assert_eq!(r.sin.len(), r.cos.len(), "table size");
+                (r.sin.f32_ptr(), r.cos.f32_ptr(), r.sin.len() / dim, r.prefix, r.tokens_per_frame)
+            }
+            None => (ptr::null(), ptr::null(), 0, 0, 0),
+        };
+        let g = self.lock();
+        expect(
+            unsafe {
+                ffi::hs_kv_append(g.0, q_ptr, k.ptr, v.ptr, q_out, k_rot, cache.k.ptr, cache.v.ptr,
+                                  cache.block_table.ptr(), kv_lens.ptr(), cu_new.map_or(ptr::null(), |c| c.ptr()), 0, 0,
+                                  0, n as u32, cache.n_seqs as u32, hq, hkv, d, pages, page, max_pages,
+                                  k.dtype.code(), sin, cos, rows as u32, prefix as u32, tpf as u32)
+            },
+            "kv_append",
+        );
+    }
+
+    /// Attention of packed sequences: q (tokens, heads, D) against k, v (tokens, kv_heads, D).
+    pub fn attention_varlen(&self, q: &CudaTensor, k: &CudaTensor, v: &CudaTensor, cu_q: &Indices,
+                            cu_k: Option<&Indices>, causal: bool) -> CudaTensor {
+        let [t, hq, d] = q.shape[..] else { panic!("attention_varlen wants (tokens,heads,D)") };
+        let [tk, hkv, dk] = k.shape[..] else { panic!("attention_varlen wants (tokens,heads,D)") };
+        assert_eq!(k.shape, v.shape);
+        assert!(dk == d && hkv > 0 && hq % hkv == 0, "heads or head_dim");
+        assert!(q.dtype == k.dtype && q.dtype == v.dtype, "attention_varlen: mixed dtypes");
+        assert!(!cu_q.is_empty() && cu_k.map_or(tk == t, |c| c.len() == cu_q.len()), "offsets");
+        let out = self.empty(&q.shape, q.dtype).unwrap_or_else(|e| panic!("attention_varlen: {e}"));
+        let g = self.lock();
+        expect(
+            unsafe {
+                ffi::hs_attention_varlen(g.0, q.ptr, k.ptr, v.ptr, out.ptr, 0, 0, 0, cu_q.ptr(),
+                                         cu_k.map_or(ptr::null(), |c| c.ptr()), t as u32, tk as u32,
+                                         (cu_q.len() - 1) as u32, hq as u32, hkv as u32, d as u32, causal as c_int,
+                                         q.dtype.code(), 0.0)
+            },
+            "attention_varlen",
+        );
+        out
+    }
+
+    /// A zeroed workspace for `attention_paged` (bytes as f32 words).  One per stream of calls.
+    pub fn paged_workspace(&self) -> Result<CudaTensor, Error> {
+        let mut bytes = 0usize;
+        {
+            let g = self.lock();
+            check(unsafe { ffi::hs_attention_paged_workspace(g.0, &mut bytes) })?;
+        }
+        let ws = self.empty(&[bytes.div_ceil(4)], Dtype::F32)?;
+        {
+            let g = self.lock();
+            check(unsafe { ffi::hs_memset(g.0, ws.ptr, 0, ws.byte_len()) })?;
+        }
+        Ok(ws)
+    }
+
+    /// One new token per sequence, q (n_seqs, heads, D), over the first kv_lens[s] cached tokens.
+    pub fn attention_paged(&self, q: &CudaTensor, cache: &PagedKv, kv_lens: &Indices, workspace: &CudaTensor)
+                           -> CudaTensor {
+        let [n, hq, dim] = q.shape[..] else { panic!("attention_paged wants (n_seqs,heads,D)") };
+        let (pages, hkv, page, d, max_pages) = cache.dims(kv_lens);
+        assert!(n == cache.n_seqs && dim as u32 == d && q.dtype == cache.k.dtype, "attention_paged: q");
+        let out = self.empty(&q.shape, q.dtype).unwrap_or_else(|e| panic!("attention_paged: {e}"));
+        let g = self.lock();
+        expect(
+            unsafe {
+                ffi::hs_attention_paged(g.0, q.ptr, out.ptr, cache.k.ptr, cache.v.ptr, cache.block_table.ptr(),
+                                        kv_lens.ptr(), 0, n as u32, hq as u32, hkv, d, pages, page, max_pages,
+                                        q.dtype.code(), 0.0, workspace.ptr, workspace.byte_len())
+            },
+            "attention_paged",
+        );
+        out
+    }
+}
+
 /// A device tensor: pool allocation + shape + dtype (GpuTensor, src/engine/tensor.rs:27-31).
 pub struct CudaTensor {
     ptr: *mut c_void,
