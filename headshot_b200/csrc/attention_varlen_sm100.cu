@@ -33,16 +33,17 @@
 // 3 % of the speed at 128 and 3 % at 64) and accumulators are f32.
 //
 // What bounds it (8,192 tokens, 32/8 x 128, not causal, one burst at 1,965 MHz:
-// 854 us, 1,288 TFLOP/s): per pair of 128 x 64 tiles about 1,900 cycles, of
+// 838 us, 1,312 TFLOP/s): per pair of 128 x 64 tiles about 1,850 cycles, of
 // which the tensor core's share is 1,260 (64-column score products run at two
-// thirds of its rate) and the MUFU's 900.  A softmax warp spends 1,070 of them
-// in the exponentials, both warpgroups at the same time and so at half the
-// MUFU's rate each, 290 in the maximum and 220 waiting for scores.  Under load
-// the 1,000 W cap takes the clock to 1,600 MHz: 1,168 TFLOP/s for a causal
-// prompt of 16,384.  Head_dim 64 is bound by the exponentials as
-// attn_fwd_sm100 is: 790 TFLOP/s for 16,384 tokens, 16 x 64, not causal.
-// Built, measured and not kept (8,192 / 16,384 tokens as above, against 1,215
-// and 790 TFLOP/s on the same GPUs):
+// thirds of its rate) and the MUFU's 900.  A softmax warp spends most of them
+// in the exponentials (both warpgroups at the same time, so at half the MUFU's
+// rate each), the rest in the maximum, in waits for scores and in the hand-over.
+// Under load the 1,000 W cap takes the clock to 1,550 MHz: 1,189 TFLOP/s for a
+// causal prompt of 16,384.  Head_dim 64 is bound by the exponentials as
+// attn_fwd_sm100 is: 848 TFLOP/s for 16,384 tokens, 16 x 64, not causal.
+// Steps kept, on these two in TFLOP/s: 1,215 / 790 -> tested waits 1,240 / 798
+// -> the next K/V tile awaited before P 1,278 / 825 -> P stored 16 columns at
+// a time 1,312 / 848.  Built and not kept, against the 1,215 / 790:
 //   head_dim 128 with 128-key tiles and one score buffer (1,079; with one MMA
 //     warp for both warpgroups 1,170, without splitting P's hand-over 1,251 in
 //     a burst, 1,052 against 1,141 at the power cap)
@@ -50,7 +51,6 @@
 //   the warpgroups' exponentials taking turns (1,175 / 720)
 //   each tile's exponentials interleaved with the next one's maximum, three
 //     64-key score buffers at head_dim 64 (806 / 748)
-//   the next K/V tile awaited before P instead of after (1,175 / 768)
 //   four MMAs per election (1,214 / 781 to 801)
 #include <cuda.h>
 
@@ -87,9 +87,9 @@ struct Shape {
   static constexpr int kSlotBytes = 2 * kKvTileBytes;
   static constexpr uint32_t kQHalf = kBM * 128;   // bytes from one column block to the next
   static constexpr uint32_t kKvHalf = kBN * 128;
-  // Of every 8 exponential pairs, this many run on the FMA pipe.  8,192 tokens
-  // of 32/8 x 128 (0, 1, 2 of 8): 1138, 1168, 1135 TFLOP/s at the power cap;
-  // 16,384 of 16 x 64 (0, 1, 2, 3): 675, 722, 727, 731.
+  // Of every 8 exponential pairs, this many run on the FMA pipe.  16,384 causal
+  // tokens of 32/8 x 128 at the power cap: 0 of 8 1,133, 1 1,189, 2 1,135
+  // TFLOP/s (an earlier build); 16,384 of 16 x 64 in a burst: 2 848, 3 820.
   static constexpr int kEmuPer8 = D == 64 ? 2 : 1;
   __host__ __device__ static constexpr uint32_t col_s(int wg, int buf) { return static_cast<uint32_t>((2 * wg + buf) * kBN); }
   __host__ __device__ static constexpr uint32_t col_o(int wg) { return static_cast<uint32_t>(4 * kBN + D * wg); }
@@ -183,8 +183,11 @@ struct RingPos {
   }
 };
 
+// Bounded wait whose outcome is the same for all 32 lanes.  Tests first: a
+// phase that is complete, the common case, costs one test and a vote (+2 %).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
                                           int site, uint64_t timeout_ns) {
+  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
   const bool r = mbar_wait(bar, parity, abort_flag, status, site, timeout_ns);
   return __all_sync(0xffffffffu, r);
 }
@@ -341,9 +344,8 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
         }
         pk[i] = Elem<E>::pack2(p0, p1);
         add2(acc[2 * (i & 1)], acc[2 * (i & 1) + 1], acc[2 * (i & 1)], acc[2 * (i & 1) + 1], p0, p1);
-        if (i == 31) tmem_st32(tS, pk);
+        if (i % 16 == 15) tmem_st16(tS + i - 15, pk + i - 15);
       }
-      if constexpr (S::kPairs == 48) tmem_st16(tS + 32, pk + 32);
       l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
       // O rescale (rare), once PV(j-1) has landed: committed with S(j+1) when
       // that tile exists, else (j = n-1) as the item's first PV-only batch.
@@ -723,6 +725,11 @@ __device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sKv, Ctrl<
         const uint32_t st = pv_pos.slot;  // V_j: waited on before S(j) was issued
         pv_pos.next();
         if (j + 1 == n && tail < kBN) clear_tail(st, tail);
+        // The next score product's tile, waited for while P(j) is still being made.
+        if (j + 2 < n && !kv_wait(s_pos)) {
+          ok = false;
+          break;
+        }
         if (!warp_wait(&ctl->p_full[wg][b], ((b ? p_base1 : p_base0) + (j >> 1)) & 1, abort_flag, a.status,
                        kSitePFull, a.timeout_ns)) {
           ok = false;
@@ -731,10 +738,6 @@ __device__ void mma_role(const Args& a, int wg, uint8_t* sQ, uint8_t* sKv, Ctrl<
         tc_fence_after();
         issue_pv(st, b, j > 0);
         if (j + 2 < n) {
-          if (!kv_wait(s_pos)) {
-            ok = false;
-            break;
-          }
           issue_s(q_desc, s_pos.slot, b);  // after PV(j) in this warp's order: P(j) is read first
           s_pos.next();
           umma_commit_elect(&ctl->s_full[wg][b]);
