@@ -89,7 +89,8 @@ HS_API hs_status hs_ctx_clear_cancel(hs_ctx* ctx);
  * when enabled, every kernel launch is bracketed by CUDA events on its
  * stream.  hs_prof_read synchronises and returns the summed device time and
  * launch count of `kernel` ("attention", "qk_prep", "layernorm",
- * "rope_apply", "permute", or "*" for all). */
+ * "rope_apply", "permute", "kv_append", "attention_varlen",
+ * "attention_paged", ..., or "*" for all). */
 HS_API hs_status hs_prof_enable(hs_ctx* ctx, int on);
 HS_API hs_status hs_prof_reset(hs_ctx* ctx);
 HS_API hs_status hs_prof_read(hs_ctx* ctx, const char* kernel, double* total_ms, uint64_t* launches);
@@ -243,7 +244,8 @@ HS_API hs_status hs_attn_merge(hs_ctx* ctx, const void* x, void* out, uint32_t S
  * kernel runs, so a captured graph follows their current values.  kv_lens[s]
  * is the length of sequence s with the tokens of the running step.  An index
  * that points outside its tensors is skipped, never followed: hs_sync then
- * returns HS_ERR_INVALID and names it. */
+ * returns HS_ERR_INVALID and names it, and the results of the sequence that
+ * holds it are unspecified. */
 
 /* Appends n_tokens new keys and values to the cache.  cu_new (n_seqs + 1,
  * rising from 0): sequence s owns tokens [cu_new[s], cu_new[s+1]), the last

@@ -306,6 +306,57 @@ def test_varlen_long(gpu_ctx):
     packed_check(out[9001:], q[9001:], k[9001:], v[9001:], lens[1:], lens[1:], True, "bf16")
 
 
+def test_varlen_many_sequences(gpu_ctx):
+    """More sequences than the scheduler scans at once, empty ones and every length class among them."""
+    for n_seqs, longest, causal in ((33, 700, True), (1500, 5, True), (200, 300, False)):
+        g = gen(n_seqs)
+        qlens = torch.randint(0, longest + 1, (n_seqs,), generator=g, device="cuda").tolist()
+        extra = torch.randint(0, 60, (n_seqs,), generator=g, device="cuda").tolist()
+        klens = [max(0, a + b - 20) for a, b in zip(qlens, extra)]
+        q = normal(g, sum(qlens), 4, 64)
+        k, v = normal(g, sum(klens), 2, 64), normal(g, sum(klens), 2, 64)
+        out = gpu_ctx.attention_varlen(q, k, v, offsets(qlens), cu_k=offsets(klens), causal=causal)
+        gpu_ctx.sync()
+        packed_check(out, q, k, v, qlens, klens, causal, "bf16")
+
+
+@pytest.mark.parametrize("hq,hkv", [(128, 1), (100, 1), (96, 2), (1, 1)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_varlen_group_extremes(gpu_ctx, hq, hkv, d):
+    g = gen(hq)
+    lens = [3, 77, 200]
+    q, k, v = normal(g, 280, hq, d), normal(g, 280, hkv, d), normal(g, 280, hkv, d)
+    out = gpu_ctx.attention_varlen(q, k, v, offsets(lens))
+    gpu_ctx.sync()
+    packed_check(out, q, k, v, lens, lens, True, "bf16")
+
+
+def test_varlen_no_keys_at_all(gpu_ctx):
+    q = normal(gen(14), 70, 4, 128)
+    none = q[:0, :2]
+    for causal in (True, False):
+        out = gpu_ctx.attention_varlen(q, none, none, offsets([30, 40]), cu_k=offsets([0, 0]), causal=causal)
+        gpu_ctx.sync()
+        assert (out == 0).all()
+
+
+def test_nan_query_stays_in_its_row(gpu_ctx):
+    g = gen(15)
+    q, k, v = normal(g, 300, 4, 64), normal(g, 300, 2, 64), normal(g, 300, 2, 64)
+    clean = gpu_ctx.attention_varlen(q, k, v, offsets([300]))
+    q[123, 2] = math.nan
+    out = gpu_ctx.attention_varlen(q, k, v, offsets([300]))
+    lens = [900, 40]
+    p, cache = paged_case(g, 8, 2, 128, 16, lens, "f16")
+    p_clean = gpu_ctx.attention_paged(p, cache, ints(lens))
+    p[0, 5] = math.nan
+    p_out = gpu_ctx.attention_paged(p, cache, ints(lens))
+    gpu_ctx.sync()
+    assert out[123, 2].isnan().all() and p_out[0, 5].isnan().all()
+    out[123, 2], p_out[0, 5] = clean[123, 2], p_clean[0, 5]
+    assert torch.equal(out, clean) and torch.equal(p_out, p_clean)
+
+
 def test_varlen_bad_offsets_are_reported(gpu_ctx):
     g = gen(12)
     q, k, v = normal(g, 40, 4, 64), normal(g, 40, 4, 64), normal(g, 40, 4, 64)
@@ -408,6 +459,29 @@ def test_paged_many_sequences_one_workspace(gpu_ctx):
         gpu_ctx.sync()
         paged_check(out, q, cache, lens, "bf16")
     assert before.numel() == ws.numel()
+
+
+def test_paged_idle_slots_and_thousands_of_sequences(gpu_ctx):
+    g = gen(25)
+    lens = torch.randint(0, 30, (5000,), generator=g, device="cuda").tolist()
+    q, cache = paged_case(g, 2, 1, 64, 16, lens, "bf16")
+    given = [-7 if n == 0 else n for n in lens]  # any length below one is an idle slot
+    out = gpu_ctx.attention_paged(q, cache, ints(given))
+    gpu_ctx.sync()
+    paged_check(out[:300], q[:300], cache, lens[:300], "bf16")
+    paged_check(out[-100:], q[-100:], PagedKv(cache.k, cache.v, cache.block_table[-100:]), lens[-100:], "bf16")
+    assert (out[[i for i, n in enumerate(lens) if n == 0]] == 0).all()
+
+
+@pytest.mark.parametrize("hq,hkv", [(48, 1), (17, 1), (128, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_paged_more_heads_than_one_tile(gpu_ctx, hq, hkv, d):
+    g = gen(hq + d)
+    lens = [2000, 5, 64]
+    q, cache = paged_case(g, hq, hkv, d, 32, lens, "bf16")
+    out = gpu_ctx.attention_paged(q, cache, ints(lens))
+    gpu_ctx.sync()
+    paged_check(out, q, cache, lens, "bf16")
 
 
 def test_paged_strided_queries_and_scale(gpu_ctx):
