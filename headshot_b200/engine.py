@@ -197,11 +197,14 @@ class GpuContext:
 
     # -------------------------------------------------------- serving ----
 
+    # These run once per token and layer: few attribute reads, few calls.
+
     def _check_rows(self, x: torch.Tensor, name: str) -> tuple[int, int, int, int]:
         """x (tokens, heads, D) with whole (heads, D) rows: its sizes and its token stride in elements."""
-        assert x.dim() == 3, f"{name} wants (tokens, heads, D)"
+        shape = x.shape
+        assert len(shape) == 3, f"{name} wants (tokens, heads, D)"
         assert x.get_device() == self._index, f"{name} must live on {self.device}"
-        t, h, d = x.shape
+        t, h, d = shape
         if x.is_contiguous():
             return t, h, d, h * d
         st, sh, sd = x.stride()
@@ -212,26 +215,27 @@ class GpuContext:
         return t, h, d, st
 
     def _check_index(self, x: torch.Tensor, name: str, shape: tuple) -> None:
-        assert x.dtype is torch.int32, f"{name} must be int32"
-        assert x.shape == shape, f"{name} must have shape {shape}"
-        self._check_tensor(x, name)
+        assert x.dtype is torch.int32 and x.shape == shape, f"{name} must be int32 of shape {shape}"
+        assert x.get_device() == self._index and x.is_contiguous(), f"{name} must be contiguous on {self.device}"
 
     def _check_cache(self, cache: PagedKv, kv_lens: torch.Tensor, dtype: torch.dtype) -> tuple:
         """(n_seqs, max_pages, pages, kv_heads, page_size, D)."""
         k, v, table = cache.k, cache.v, cache.block_table
-        assert k.dim() == 4 and k.shape == v.shape, "cache wants k, v (pages, heads, page_size, D)"
+        shape, tshape = k.shape, table.shape
+        assert len(shape) == 4 and v.shape == shape, "cache wants k, v (pages, heads, page_size, D)"
         assert k.dtype is dtype and v.dtype is dtype, "cache dtype mismatch"
-        assert table.dim() == 2, "block_table wants (n_seqs, max_pages)"
-        n_seqs, max_pages = table.shape
-        self._check_tensor(k, "cache.k")
-        self._check_tensor(v, "cache.v")
-        self._check_index(table, "block_table", (n_seqs, max_pages))
-        self._check_index(kv_lens, "kv_lens", (n_seqs,))
-        return n_seqs, max_pages, *k.shape
+        assert len(tshape) == 2 and table.dtype is torch.int32, "block_table wants int32 (n_seqs, max_pages)"
+        assert kv_lens.dtype is torch.int32 and kv_lens.shape == tshape[:1], "kv_lens wants int32 (n_seqs,)"
+        i = self._index
+        assert k.get_device() == i and v.get_device() == i and table.get_device() == i and kv_lens.get_device() == i, \
+            f"cache, block_table and kv_lens must live on {self.device}"
+        assert k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and kv_lens.is_contiguous(), \
+            "cache, block_table and kv_lens must be contiguous"
+        return *tshape, *shape
 
     def _check_out(self, out: torch.Tensor, like: torch.Tensor, name: str) -> None:
         assert out.shape == like.shape and out.dtype is like.dtype, f"{name} shape"
-        self._check_tensor(out, name)
+        assert out.get_device() == self._index and out.is_contiguous(), f"{name} must be contiguous on {self.device}"
 
     def kv_append(self, cache: PagedKv, k: torch.Tensor, v: torch.Tensor, kv_lens: torch.Tensor,
                   cu_new: torch.Tensor | None = None, rope: Rope | None = None, q: torch.Tensor | None = None,
@@ -274,8 +278,8 @@ class GpuContext:
             sin, cos = rope.sin, rope.cos
             assert sin.dtype is torch.float32 and cos.dtype is torch.float32, "rope tables must be f32"
             assert sin.shape == cos.shape and sin.shape[-1] == d, "table size"
-            self._check_tensor(sin, "rope.sin")
-            self._check_tensor(cos, "rope.cos")
+            assert sin.get_device() == self._index and cos.get_device() == self._index and sin.is_contiguous() \
+                and cos.is_contiguous(), f"rope tables must be contiguous on {self.device}"
             rows, prefix, tpf = sin.numel() // d, rope.prefix, rope.tokens_per_frame or 0
         if n == 0 or n_seqs == 0:
             return q_out
