@@ -33,14 +33,19 @@
 // 3 % of the speed at 128 and 3 % at 64) and accumulators are f32.
 //
 // What bounds it (8,192 tokens, 32/8 x 128, not causal, one burst at 1,965 MHz:
-// 838 us, 1,312 TFLOP/s): per pair of 128 x 64 tiles about 1,850 cycles, of
+// 825 us, 1,333 TFLOP/s): per pair of 128 x 64 tiles about 1,850 cycles, of
 // which the tensor core's share is 1,260 (64-column score products run at two
 // thirds of its rate) and the MUFU's 900.  A softmax warp spends most of them
 // in the exponentials (both warpgroups at the same time, so at half the MUFU's
 // rate each), the rest in the maximum, in waits for scores and in the hand-over.
 // Under load the 1,000 W cap takes the clock to 1,550 MHz: 1,189 TFLOP/s for a
 // causal prompt of 16,384.  Head_dim 64 is bound by the exponentials as
-// attn_fwd_sm100 is: 848 TFLOP/s for 16,384 tokens, 16 x 64, not causal.
+// attn_fwd_sm100 is: 848 TFLOP/s for 16,384 tokens, 16 x 64, not causal.  An
+// item's start and end cost about 6,000 cycles, three 96-key tiles' worth, and
+// the GPU hands out about 28 pending blocks a microsecond, which bounds
+// thousands of items that are shorter than 5 us each.  (Dealing half to seven
+// eighths of the items out by block index instead: 9 % faster there, up to
+// 7 % slower on ragged prompts.)
 // Steps kept, on these two in TFLOP/s: 1,215 / 790 -> tested waits 1,240 / 798
 // -> the next K/V tile awaited before P 1,278 / 825 -> P stored 16 columns at
 // a time 1,312 / 848.  Built and not kept, against the 1,215 / 790:
@@ -164,6 +169,7 @@ struct Args {
   uint32_t kv_heads;
   uint32_t tile_tokens;  // tokens per 128-row tile: 128 / group
   int causal;
+  int out_sectors;  // out is 32-byte aligned
   float scale_log2;
   int* status;
   uint64_t timeout_ns;
@@ -253,6 +259,12 @@ __device__ __forceinline__ void exp2_poly2(float x0, float x1, float& y0, float&
   fma2(p0, p1, p0, p1, f0, f1, kExpC0, kExpC0);
   y0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
   y1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+}
+
+__device__ __forceinline__ void store32(void* dst, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 template <typename E, int D>
@@ -391,17 +403,20 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
         tmem_wait_ld_regs<32>(o);
       }
       if (valid) {
-        uint4* dst = reinterpret_cast<uint4*>(out + 32 * h);
+        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (!empty) {
-            v.x = Elem<E>::pack2(u2f(o[8 * i + 0]) * inv_l, u2f(o[8 * i + 1]) * inv_l);
-            v.y = Elem<E>::pack2(u2f(o[8 * i + 2]) * inv_l, u2f(o[8 * i + 3]) * inv_l);
-            v.z = Elem<E>::pack2(u2f(o[8 * i + 4]) * inv_l, u2f(o[8 * i + 5]) * inv_l);
-            v.w = Elem<E>::pack2(u2f(o[8 * i + 6]) * inv_l, u2f(o[8 * i + 7]) * inv_l);
-          }
-          dst[i] = v;
+        for (int i = 0; i < 16; ++i)
+          w[i] = empty ? 0u : Elem<E>::pack2(u2f(o[2 * i]) * inv_l, u2f(o[2 * i + 1]) * inv_l);
+        // The lanes' rows lie apart, so a store's cost is the sectors it touches:
+        // whole 32-byte ones where the base allows (400 sequences of 256 tokens,
+        // 16 x 64: 284 -> 262 us).
+        if (a.out_sectors) {
+          store32(out + 32 * h, w);
+          store32(out + 32 * h + 16, w + 8);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            reinterpret_cast<uint4*>(out + 32 * h)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         }
       }
     }
@@ -896,6 +911,7 @@ cudaError_t launch_attention_varlen(cudaStream_t stream, int code, uint32_t d, c
   a.kv_heads = io.kv_heads;
   a.tile_tokens = kBM / a.group;
   a.causal = io.causal;
+  a.out_sectors = (reinterpret_cast<uintptr_t>(io.out) & 31u) == 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = status;
   a.timeout_ns = timeout_ns;

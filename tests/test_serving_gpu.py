@@ -306,6 +306,20 @@ def test_varlen_long(gpu_ctx):
     packed_check(out[9001:], q[9001:], k[9001:], v[9001:], lens[1:], lens[1:], True, "bf16")
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_varlen_output_aligned_to_16_bytes_only(gpu_ctx, d):
+    g = gen(16)
+    lens = [130, 7]
+    q, k, v = normal(g, 137, 6, d), normal(g, 137, 2, d), normal(g, 137, 2, d)
+    buf = torch.full((137 * 6 * d + 16,), 2.0, dtype=torch.bfloat16, device="cuda")
+    out = buf[8:8 + 137 * 6 * d].view(137, 6, d)
+    assert out.data_ptr() % 32 == 16
+    gpu_ctx.attention_varlen(q, k, v, offsets(lens), out=out)
+    want = gpu_ctx.attention_varlen(q, k, v, offsets(lens))
+    gpu_ctx.sync()
+    assert torch.equal(out, want) and (buf[:8] == 2).all() and (buf[-8:] == 2).all()
+
+
 def test_varlen_many_sequences(gpu_ctx):
     """More sequences than the scheduler scans at once, empty ones and every length class among them."""
     for n_seqs, longest, causal in ((33, 700, True), (1500, 5, True), (200, 300, False)):
