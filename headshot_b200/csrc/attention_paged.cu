@@ -196,59 +196,49 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, S
   return total;
 }
 
-// Issues this warp's keys of a tile into its ring stage.
-template <typename E, int D, bool kWholeSteps>
+// Issues this warp's keys of a tile into its ring stage.  Lane r looks up the
+// cache row of key r of 16, whatever the page size, and the copies take the
+// rows from the lanes (one look-up for all 16 where a page holds them gains
+// nothing that is measurable: 274,800 keys, 16 x 64, 170.5 us against 171.5; 128
+// ragged sequences, 32/8 x 128, 166.0 against 164.6).
+template <typename E, int D>
 __device__ __forceinline__ void load_tile(const Args& a, const Place& p, uint32_t stage, int warp, int lane) {
   using S = Shape<D>;
   constexpr int kChunks = D / 8;            // 16-byte chunks per row
   constexpr int kRowsPer = 32 / kChunks;    // rows one warp instruction covers
   const uint32_t key0 = p.tile * S::kTileKeys + warp * S::kWarpKeys;
-  if (key0 >= p.len) return;
+  if (key0 >= p.len) return;  // the same for the whole warp
   const uint32_t chunk = lane % kChunks;
   const uint32_t head = p.sub / a.head_tiles;
   const int* table = a.c.table + static_cast<uint64_t>(p.seq) * a.c.max_pages;
   const E* kc = static_cast<const E*>(a.c.k) + 8 * chunk;
   const E* vc = static_cast<const E*>(a.c.v) + 8 * chunk;
-  // Element offset of cache row 0 of the page that holds `key`; ok: it exists.
-  auto page_row = [&](uint32_t key, uint32_t* off, bool* ok) -> uint64_t {
-    const uint32_t slot = key / a.c.page_size;
-    *off = key - slot * a.c.page_size;
-    int page = __ldg(table + slot);
-    if (page < 0 || static_cast<uint32_t>(page) >= a.c.n_pages) {
-      atomicCAS(a.status, 0, static_cast<int>(kSiteBadPage));
-      *ok = false;
-      page = 0;
-    }
-    return (static_cast<uint64_t>(page) * a.c.heads + head) * a.c.page_size;
-  };
 #pragma unroll
   for (int step = 0; step < S::kWarpKeys; step += 16) {
-    bool page_ok = key0 + step < p.len;
-    uint32_t off0 = 0;
-    uint64_t row0 = 0;
-    if (kWholeSteps && page_ok) row0 = page_row(key0 + step, &off0, &page_ok);  // 16 keys never straddle pages
+    const uint32_t key = key0 + step + (lane & 15);
+    uint64_t row = ~0ull;  // of the cache, in rows of D; all ones: no such key
+    if (key < p.len) {
+      const uint32_t slot = key / a.c.page_size;
+      const int page = __ldg(table + slot);
+      if (page < 0 || static_cast<uint32_t>(page) >= a.c.n_pages)
+        atomicCAS(a.status, 0, static_cast<int>(kSiteBadPage));
+      else
+        row = (static_cast<uint64_t>(page) * a.c.heads + head) * a.c.page_size + (key - slot * a.c.page_size);
+    }
 #pragma unroll
     for (int i = 0; i < 16 / kRowsPer; ++i) {
-      const uint32_t r = step + i * kRowsPer + lane / kChunks;
-      bool ok = key0 + r < p.len;
-      uint64_t at;
-      if (kWholeSteps) {
-        ok = ok && page_ok;
-        at = (row0 + off0 + r - step) * D;
-      } else {
-        uint32_t off = 0;
-        at = ok ? page_row(key0 + r, &off, &ok) : 0;
-        at = (at + off) * D;
-      }
-      if (!ok) at = 0;
-      const uint32_t dst = stage + r * (D * 2) + ((chunk ^ (r & 7)) << 4);
+      const uint32_t r = i * kRowsPer + lane / kChunks;  // of the step
+      const uint64_t from = __shfl_sync(0xffffffffu, row, static_cast<int>(r));
+      const bool ok = from != ~0ull;
+      const uint64_t at = ok ? from * D : 0;
+      const uint32_t dst = stage + (step + r) * (D * 2) + ((chunk ^ (r & 7)) << 4);
       cp_async16(dst, kc + at, ok);
       cp_async16(dst + S::kWarpKeys * D * 2, vc + at, ok);
     }
   }
 }
 
-template <typename E, int D, bool kWholeSteps>
+template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_paged_kernel(const __grid_constant__ Args a) {
   using S = Shape<D>;
   extern __shared__ __align__(128) uint8_t ring[];
@@ -307,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
   uint32_t load_stage = 0;
   auto load_next = [&] {
     if (ahead.at < end) {
-      load_tile<E, D, kWholeSteps>(a, ahead, my_ring + load_stage * S::kStageBytes, warp, lane);
+      load_tile<E, D>(a, ahead, my_ring + load_stage * S::kStageBytes, warp, lane);
       next_tile<D>(a, ahead);
     }
     load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
@@ -544,10 +534,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
   cp_async_wait<0>();
 }
 
-template <typename E, int D, bool kWholeSteps>
+template <typename E, int D>
 cudaError_t launch(cudaStream_t stream, const Args& a) {
   using S = Shape<D>;
-  const void* f = reinterpret_cast<const void*>(attention_paged_kernel<E, D, kWholeSteps>);
+  const void* f = reinterpret_cast<const void*>(attention_paged_kernel<E, D>);
   const cudaError_t e = ensure_dynamic_smem(f, S::kSmem);
   if (e != cudaSuccess) return e;
   uint64_t ctas = static_cast<uint64_t>(current_sm_count()) * S::kCtasPerSm;
@@ -556,14 +546,8 @@ cudaError_t launch(cudaStream_t stream, const Args& a) {
   const uint64_t most = (static_cast<uint64_t>(a.c.max_pages) * a.c.page_size + S::kTileKeys - 1) / S::kTileKeys;
   const uint64_t tiles = static_cast<uint64_t>(a.c.n_seqs) * a.subs * (most ? most : 1);
   if (ctas > (tiles + S::kMinTiles - 1) / S::kMinTiles) ctas = (tiles + S::kMinTiles - 1) / S::kMinTiles;
-  attention_paged_kernel<E, D, kWholeSteps><<<static_cast<uint32_t>(ctas), kThreads, S::kSmem, stream>>>(a);
+  attention_paged_kernel<E, D><<<static_cast<uint32_t>(ctas), kThreads, S::kSmem, stream>>>(a);
   return cudaGetLastError();
-}
-
-template <typename E, int D>
-cudaError_t launch_pages(cudaStream_t stream, const Args& a) {
-  // Pages of a multiple of 16 keys: one table entry serves 16 keys.
-  return a.c.page_size % 16 == 0 ? launch<E, D, true>(stream, a) : launch<E, D, false>(stream, a);
 }
 
 }  // namespace
@@ -585,8 +569,8 @@ cudaError_t launch_attention_paged(cudaStream_t stream, int code, uint32_t d, co
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = status;
   if (code == kBF16)
-    return d == 64 ? launch_pages<__nv_bfloat16, 64>(stream, a) : launch_pages<__nv_bfloat16, 128>(stream, a);
-  return d == 64 ? launch_pages<__half, 64>(stream, a) : launch_pages<__half, 128>(stream, a);
+    return d == 64 ? launch<__nv_bfloat16, 64>(stream, a) : launch<__nv_bfloat16, 128>(stream, a);
+  return d == 64 ? launch<__half, 64>(stream, a) : launch<__half, 128>(stream, a);
 }
 
 }  // namespace hs

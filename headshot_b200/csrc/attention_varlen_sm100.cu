@@ -115,7 +115,7 @@ enum : int {
   kSiteNext = 0x30a,
 };
 
-// One unit of work, as the producer decodes it.
+// One unit of work, as the scheduler decodes it.
 struct Item {
   int q_row;     // first query token of the item, in the packed rows; kNoItem: no more work
   int tokens;    // query tokens from there to the sequence's end (may exceed the item)

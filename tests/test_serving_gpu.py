@@ -444,6 +444,8 @@ def paged_check(out, q, cache, lens, dtype, scale=None):
     (100, [99, 100, 101, 777]),
     (64, [5000]),
     (256, [4099, 1, 300]),
+    (8, [37, 1000]),
+    (12, [11, 12, 13, 600]),
 ])
 def test_paged(gpu_ctx, dtype, hq, hkv, d, page, lens):
     g = gen(page + hq + d)
