@@ -33,14 +33,14 @@
 // 3 % of the speed at 128 and 3 % at 64) and accumulators are f32.
 //
 // What bounds it (8,192 tokens, 32/8 x 128, not causal, one burst at 1,965 MHz:
-// 825 us, 1,333 TFLOP/s): per pair of 128 x 64 tiles about 1,850 cycles, of
+// 827 us, 1,329 TFLOP/s): per pair of 128 x 64 tiles about 1,850 cycles, of
 // which the tensor core's share is 1,260 (64-column score products run at two
 // thirds of its rate) and the MUFU's 900.  A softmax warp spends most of them
 // in the exponentials (both warpgroups at the same time, so at half the MUFU's
 // rate each), the rest in the maximum, in waits for scores and in the hand-over.
 // Under load the 1,000 W cap takes the clock to 1,550 MHz: 1,189 TFLOP/s for a
 // causal prompt of 16,384.  Head_dim 64 is bound by the exponentials as
-// attn_fwd_sm100 is: 848 TFLOP/s for 16,384 tokens, 16 x 64, not causal.  An
+// attn_fwd_sm100 is: 837 TFLOP/s for 16,384 tokens, 16 x 64, not causal.  An
 // item's start and end cost about 6,000 cycles, three 96-key tiles' worth, and
 // the GPU hands out about 28 pending blocks a microsecond, which bounds
 // thousands of items that are shorter than 5 us each.  (Dealing half to seven
@@ -48,7 +48,8 @@
 // 7 % slower on ragged prompts.)
 // Steps kept, on these two in TFLOP/s: 1,215 / 790 -> tested waits 1,240 / 798
 // -> the next K/V tile awaited before P 1,278 / 825 -> P stored 16 columns at
-// a time 1,312 / 848.  Built and not kept, against the 1,215 / 790:
+// a time 1,312 / 830 -> the FMA pipe's share last of each 16 pairs, masked
+// weights exactly zero 1,329 / 837.  Built and not kept, against the 1,215 / 790:
 //   head_dim 128 with 128-key tiles and one score buffer (1,079; with one MMA
 //     warp for both warpgroups 1,170, without splitting P's hand-over 1,251 in
 //     a burst, 1,052 against 1,141 at the power cap)
@@ -92,10 +93,11 @@ struct Shape {
   static constexpr int kSlotBytes = 2 * kKvTileBytes;
   static constexpr uint32_t kQHalf = kBM * 128;   // bytes from one column block to the next
   static constexpr uint32_t kKvHalf = kBN * 128;
-  // Of every 8 exponential pairs, this many run on the FMA pipe.  16,384 causal
-  // tokens of 32/8 x 128 at the power cap: 0 of 8 1,133, 1 1,189, 2 1,135
-  // TFLOP/s (an earlier build); 16,384 of 16 x 64 in a burst: 2 848, 3 820.
-  static constexpr int kEmuPer8 = D == 64 ? 2 : 1;
+  // Of every 16 exponential pairs, the last this many run on the FMA pipe.
+  // 8,192 tokens of 32/8 x 128 in a burst: 1 of 16 1,245, 2 1,329, 3 1,292
+  // TFLOP/s; 16,384 of 16 x 64: 2 775, 4 837, 5 837, 6 822.  The same share
+  // at the start of each 16 or each 8 loses 3 to 6 %.
+  static constexpr int kEmuPer16 = D == 64 ? 4 : 2;
   __host__ __device__ static constexpr uint32_t col_s(int wg, int buf) { return static_cast<uint32_t>((2 * wg + buf) * kBN); }
   __host__ __device__ static constexpr uint32_t col_o(int wg) { return static_cast<uint32_t>(4 * kBN + D * wg); }
   static_assert(4 * kBN + 2 * D <= 512, "TMEM budget");
@@ -240,7 +242,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // 2^x for a pair on the FMA pipe: the same reduction and cubic as
-// attn_fwd_sm100's (max relative error 8.3e-5, inputs clamped at -125).
+// attn_fwd_sm100's (max relative error 8.3e-5).  Below 2^-127 the exponent sum
+// turns negative and the result is 0, as the MUFU's is below 2^-126 (add and
+// maximum are one instruction): a masked weight has to be 0 and not merely
+// tiny, since a bf16 value reaches 2^128.
 constexpr float kExpMagic = 12582912.0f;  // 1.5 * 2^23
 constexpr float kExpC0 = 0.99991959f;
 constexpr float kExpC1 = 0.69326216f;
@@ -248,8 +253,8 @@ constexpr float kExpC2 = 0.24271429f;
 constexpr float kExpC3 = 0.05521307f;
 
 __device__ __forceinline__ void exp2_poly2(float x0, float x1, float& y0, float& y1) {
-  x0 = fmaxf(x0, -125.f);
-  x1 = fmaxf(x1, -125.f);
+  x0 = fmaxf(x0, -150.f);
+  x1 = fmaxf(x1, -150.f);
   float t0, t1, r0, r1, f0, f1, p0, p1;
   add2(t0, t1, x0, x1, kExpMagic, kExpMagic);
   add2(r0, r1, t0, t1, -kExpMagic, -kExpMagic);
@@ -257,8 +262,8 @@ __device__ __forceinline__ void exp2_poly2(float x0, float x1, float& y0, float&
   fma2(p0, p1, f0, f1, kExpC3, kExpC3, kExpC2, kExpC2);
   fma2(p0, p1, p0, p1, f0, f1, kExpC1, kExpC1);
   fma2(p0, p1, p0, p1, f0, f1, kExpC0, kExpC0);
-  y0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-  y1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+  y0 = __int_as_float(__viaddmax_s32(__float_as_int(p0), __float_as_int(t0) << 23, 0));
+  y1 = __int_as_float(__viaddmax_s32(__float_as_int(p1), __float_as_int(t1) << 23, 0));
 }
 
 __device__ __forceinline__ void store32(void* dst, const uint32_t* w) {
@@ -348,7 +353,7 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
       for (int i = 0; i < S::kPairs; ++i) {
         float x0, x1, p0, p1;
         fma2(x0, x1, u2f(s[2 * i]), u2f(s[2 * i + 1]), c, c, neg_m, neg_m);
-        if ((i & 7) < S::kEmuPer8) {
+        if ((i & 15) >= 16 - S::kEmuPer16) {
           exp2_poly2(x0, x1, p0, p1);
         } else {
           p0 = ex2_approx(x0);

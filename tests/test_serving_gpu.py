@@ -291,6 +291,38 @@ def test_varlen_rising_and_extreme_scores(gpu_ctx, dtype, d):
     packed_check(out, q, k, v, [n], [n], True, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_largest_values_in_masked_places(gpu_ctx, dtype, d):
+    """The type's largest values behind a causal mask, and on keys whose score lies 200 binades down,
+    add nothing: their weights are zero, not tiny (2^-125 of bf16's largest value would be 8)."""
+    g = gen(17)
+    n, big = 200, torch.finfo(TORCH[dtype]).max
+    q, k, v = normal(g, n, 2, d, dtype=dtype), normal(g, n, 2, d, dtype=dtype), normal(g, n, 2, d, dtype=dtype)
+    v[120:] = big
+    k[120:] = -big / 1e30 if dtype == "bf16" else -big
+    out = gpu_ctx.attention_varlen(q, k, v, offsets([n]))
+    gpu_ctx.sync()
+    packed_check(out[:120], q[:120], k[:120], v[:120], [120], [120], True, dtype)
+
+    # Far below the maximum: queries of ones, keys of +-c with |q.k| scale log2 e = 100 each way.
+    one = torch.ones(n, 2, d, device="cuda").to(TORCH[dtype])
+    c = 100.0 / (d ** 0.5 * 1.4426950408889634)
+    low = torch.full_like(one, c)
+    low[1::3] = -c  # 200 binades below the others
+    w = normal(g, n, 2, d, dtype=dtype)
+    w[1::3] = big
+    for causal in (True, False):
+        out = gpu_ctx.attention_varlen(one, low, w, offsets([n]), causal=causal)
+        keep = [i for i in range(n) if i % 3 != 1]
+        gpu_ctx.sync()
+        for i in (0, 1, 5, 63, 64, 150, 199):
+            seen = [j for j in keep if not causal or j <= i]
+            want = w[seen].double().mean(0)
+            mass = w[seen].double().abs().mean(0)
+            check_attention(out[i], want, mass, n, dtype, w[seen].abs().max().item())
+
+
 def test_varlen_long(gpu_ctx):
     """Many key tiles and items per processor, ragged, against 64 bits on sampled rows."""
     g = gen(11)
