@@ -308,7 +308,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
 
   uint32_t q[D / 16][4];
   float o[D / 8][4];
-  float m[2], l[2];
+  float m[2], l[2];                   // m: running maximum of the scores, before the scale
+  const float threshold = kRescaleThreshold / a.scale_log2;
   const uint32_t row_lo = lane >> 2;  // rows row_lo and row_lo + 8 of the head tile
 
   bool fresh = true;                  // the next tile starts a segment
@@ -369,13 +370,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
         for (int x = 1; x < kCols; ++x) t = fmaxf(t, fmaxf(s[x][2 * h], s[x][2 * h + 1]));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-        top[h] = t * a.scale_log2;
+        top[h] = t;
       }
-      if (__any_sync(0xffffffffu, top[0] > m[0] + kRescaleThreshold || top[1] > m[1] + kRescaleThreshold)) {
+      if (__any_sync(0xffffffffu, top[0] > m[0] + threshold || top[1] > m[1] + threshold)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float m_new = fmaxf(m[h], top[h]);
-          const float f = m_new == -INFINITY ? 1.f : ex2_approx(m[h] - m_new);
+          const float f = m_new == -INFINITY ? 1.f : ex2_approx((m[h] - m_new) * a.scale_log2);
           m[h] = m_new;
           l[h] *= f;
 #pragma unroll
@@ -393,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float base_m = m[h] == -INFINITY ? 0.f : m[h];
-            const uint32_t w = Elem<E>::pack2(ex2_approx(fmaf(s[g + t][2 * h], a.scale_log2, -base_m)),
-                                              ex2_approx(fmaf(s[g + t][2 * h + 1], a.scale_log2, -base_m)));
+            const uint32_t w = Elem<E>::pack2(ex2_approx((s[g + t][2 * h] - base_m) * a.scale_log2),
+                                              ex2_approx((s[g + t][2 * h + 1] - base_m) * a.scale_log2));
             const float2 f = Elem<E>::unpack2(w);
             l[h] += f.x + f.y;
             p[2 * t + h] = w;
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float f = sh.m[w][r] == -INFINITY ? 0.f : ex2_approx(sh.m[w][r] - mt);
+          const float f = sh.m[w][r] == -INFINITY ? 0.f : ex2_approx((sh.m[w][r] - mt) * a.scale_log2);
           lt = fmaf(sh.l[w][r], f, lt);
           const float4 v = *reinterpret_cast<const float4*>(
               ring + (w * S::kStages + st) * S::kStageBytes +
@@ -502,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
               float m_new = mt;
 #pragma unroll
               for (uint32_t x = 0; x < kPart; ++x) m_new = fmaxf(m_new, mc[x]);
-              const float f0 = mt == -INFINITY ? 0.f : ex2_approx(mt - m_new);
+              const float f0 = mt == -INFINITY ? 0.f : ex2_approx((mt - m_new) * a.scale_log2);
               mt = m_new;
               lt *= f0;
               acc.x *= f0;
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
               acc.w *= f0;
 #pragma unroll
               for (uint32_t x = 0; x < kPart; ++x) {
-                const float f = mc[x] == -INFINITY ? 0.f : ex2_approx(mc[x] - mt);
+                const float f = mc[x] == -INFINITY ? 0.f : ex2_approx((mc[x] - mt) * a.scale_log2);
                 lt = fmaf(lc[x], f, lt);
                 acc.x = fmaf(v[x].x, f, acc.x);
                 acc.y = fmaf(v[x].y, f, acc.y);

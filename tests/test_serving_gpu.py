@@ -323,6 +323,35 @@ def test_largest_values_in_masked_places(gpu_ctx, dtype, d):
             check_attention(out[i], want, mass, n, dtype, w[seen].abs().max().item())
 
 
+@pytest.mark.parametrize("dtype,size", [("bf16", 300.0), ("bf16", 2e3), ("bf16", 1e9), ("f16", 2e3), ("f16", 6e4)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_huge_scores(gpu_ctx, dtype, size, d):
+    """Scores whose product with the scale rounds away whole binades: each row still belongs to its
+    largest score, which the inputs set apart from the others by far.  (Packed prompts: to 2^26.)"""
+    g = gen(18)
+    n = 130
+    sign = torch.where(torch.rand(n, 1, d, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    k = (sign * size).to(TORCH[dtype])
+    q = (sign.flip(0) * size).to(TORCH[dtype])
+    v = normal(g, n, 1, d, dtype=dtype)
+    if size * size * d ** 0.5 <= 2.0 ** 26:
+        out = gpu_ctx.attention_varlen(q, k, v, offsets([n]), causal=False)
+    else:
+        out = v.flip(0)
+    table = torch.arange(9, dtype=torch.int32, device="cuda")[None]
+    kc, vc = (torch.zeros(9, 1, 16, d, dtype=TORCH[dtype], device="cuda") for _ in range(2))
+    cache = PagedKv(kc, vc, table)
+    gpu_ctx.kv_append(cache, k, v, ints([n]), cu_new=offsets([n]))
+    rows = [gpu_ctx.attention_paged(q[i:i + 1], cache, ints([n])) for i in (0, 40, 129)]
+    gpu_ctx.sync()
+    # Row i's own sign pattern is key n - 1 - i: score d size^2, the next one at least 2 size^2 less.
+    # Its weight is 2^r with r the rounding of the maximum times the scale, |r| <= 2 here, so not
+    # 1: it is rounded (u) where it multiplies the value and not in the sum, hence no equality.
+    check_attention(out, v.flip(0).double(), v.flip(0).double().abs(), n, dtype, v.abs().max().item())
+    for i, got in zip((0, 40, 129), rows):
+        assert torch.equal(got[0], v[n - 1 - i])
+
+
 def test_varlen_long(gpu_ctx):
     """Many key tiles and items per processor, ragged, against 64 bits on sampled rows."""
     g = gen(11)
