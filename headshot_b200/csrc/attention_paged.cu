@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtasPerSm) attention_page
   uint32_t q[D / 16][4];
   float o[D / 8][4];
   float m[2], l[2];                   // m: running maximum of the scores, before the scale
-  const float threshold = kRescaleThreshold / a.scale_log2;
+  const float threshold = fminf(kRescaleThreshold / a.scale_log2, 1e30f);  // finite: -inf + it stays below any score
   const uint32_t row_lo = lane >> 2;  // rows row_lo and row_lo + 8 of the head tile
 
   bool fresh = true;                  // the next tile starts a segment

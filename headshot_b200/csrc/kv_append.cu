@@ -18,6 +18,9 @@
 // loads are issued before the token's place (sequence, length, page, table row)
 // is looked up, so the four dependent reads hide behind them.  An element is
 // read and written by the same thread, so q_out may be q and k_out may be k.
+//
+// Measured: 32,768 tokens, 32/8 x 128: 139 us, 6.5 TB/s (a plain copy reaches
+// 6.55); 24 ragged prompts of 8,898 tokens 41.6 us, 5.8 TB/s; one token 2.7 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -27,7 +30,10 @@
 namespace hs {
 namespace {
 
-constexpr int kThreads = 256;
+// 40 prompts of 10 to 1,500 tokens, 16/16 x 64 and 16/16 x 128: 128 threads with
+// 2, 4, 6 heads in flight 29.2, 30.0, 31.0 and 52.7, 52.3, 52.4 us; 256 threads
+// with 4 33.7 and 53.6; 64 threads like 128, but slower for single tokens.
+constexpr int kThreads = 128;
 constexpr int kBatch = 4;  // heads in flight per thread
 
 struct Args {
