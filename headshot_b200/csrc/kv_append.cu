@@ -69,6 +69,13 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   const uint32_t per_token = kChunks * lanes;  // a multiple of 32: a warp holds one token
   const uint32_t tokens = kThreads / per_token;
   const uint32_t token = blockIdx.x * tokens + threadIdx.x / per_token;
+  // A token sees the offsets of its own sequence only, so the grid shares out
+  // the neighbouring pairs, one a thread, to find the falling ones.
+  if (a.cu_new) {
+    for (uint64_t s = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; s < c.n_seqs;
+         s += static_cast<uint64_t>(gridDim.x) * kThreads)
+      if (__ldg(a.cu_new + s + 1) < __ldg(a.cu_new + s)) atomicCAS(args.status, 0, static_cast<int>(kSiteBadOffsets));
+  }
   if (token >= a.n_tokens) return;
   const uint32_t in_token = threadIdx.x % per_token;
   const uint32_t chunk = in_token % kChunks;
@@ -97,10 +104,15 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   uint32_t seq = token;
   int64_t pos;
   if (a.cu_new) {
-    if (static_cast<int>(token) >= __ldg(a.cu_new + c.n_seqs) || static_cast<int>(token) < __ldg(a.cu_new)) return;
+    const int64_t start = __ldg(a.cu_new), last = __ldg(a.cu_new + c.n_seqs);
+    const bool fits = start == 0 && last <= static_cast<int64_t>(a.n_tokens);
+    if (!fits && in_token == 0) atomicCAS(args.status, 0, static_cast<int>(kSiteBadOffsets));
+    if (token >= last || token < start) return;
     seq = find_seq(a.cu_new, c.n_seqs, static_cast<int>(token));
     const int64_t first = __ldg(a.cu_new + seq), end = __ldg(a.cu_new + seq + 1);
-    if (token < first || token >= end) {
+    // An end past the rows or past the last offset would count the token's
+    // position back from tokens that do not exist.
+    if (first < 0 || token < first || token >= end || end > last || end > static_cast<int64_t>(a.n_tokens)) {
       if (in_token == 0) atomicCAS(args.status, 0, static_cast<int>(kSiteBadOffsets));
       return;
     }

@@ -244,7 +244,8 @@ class GpuContext:
 
         Sequence s owns tokens [cu_new[s], cu_new[s+1]) (one each without cu_new), its last one at
         position kv_lens[s] - 1: kv_lens counts the tokens after the append.  Tokens whose position
-        comes out negative and tokens past cu_new[-1] are padding and left alone.  `rope` tables have
+        comes out negative and tokens past cu_new[-1] are padding and left alone; offsets that do not
+        rise from 0 within the tokens are reported by sync().  `rope` tables have
         a row per position (tokens_per_frame None) or per frame token.  With q, returns the tokens'
         rotated queries (q_out, allocated if not given); k_out receives the rotated keys once more,
         as attention_varlen takes them."""

@@ -252,6 +252,8 @@ HS_API hs_status hs_attn_merge(hs_ctx* ctx, const void* x, void* out, uint32_t S
  * of which takes position kv_lens[s] - 1; NULL: one token per sequence
  * (n_tokens == n_seqs).  A token whose position comes out negative, and
  * tokens from cu_new[n_seqs] on, are padding: nothing is written for them.
+ * Offsets that do not start at 0, that fall, or that end past n_tokens are
+ * reported by hs_sync; a sequence whose own end does not fit appends nothing.
  * Two tokens of one call must not share a cache row.
  * rope_sin != NULL rotates k, and q if given, as hs_rope_apply does: table
  * row of position p is (p mod tokens_per_frame) - prefix, p itself for

@@ -1,0 +1,80 @@
+"""The serving operators on the GPU at the places where their results, reports and promises are
+easy to miss: offsets that do not fit the packed rows, keys that are not numbers at every position of
+a tile, scores of any size, equal bits whatever the block table's width, a workspace that is ready
+for the next call, refusals by the library itself.  Tolerances as in test_serving_gpu.py."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from headshot_b200._lib import HS_ERR_INVALID, HsError
+from headshot_b200.engine import PagedKv
+from test_serving_gpu import gathered, gen, ints, normal, offsets, paged_case
+
+pytestmark = pytest.mark.gpu
+
+
+def reported(ctx, word):
+    with pytest.raises(HsError) as e:
+        ctx.sync()
+    assert e.value.status == HS_ERR_INVALID and word in e.value.message
+
+
+# -------------------------------------------------------------- kv_append --
+
+
+@pytest.mark.parametrize("cu,healthy", [
+    ([0, 20, 60], [0]),          # an end past the packed rows
+    ([0, 30, 20], []),           # falling
+    ([0, -5, 40], []),           # negative
+    ([5, 20, 40], None),         # does not start at 0: tokens 0 to 4 belong to nobody
+    ([0, 0, 2 ** 31 - 1], []),
+    ([0, 10, 41], [0]),          # one past
+    ([0, 40, 35], []),
+])
+def test_append_reports_bad_offsets_and_keeps_the_history(gpu_ctx, cu, healthy):
+    """Offsets that do not rise from 0 within the rows are reported; a sequence whose end is wrong
+    appends nothing, so its history keeps its rows, and a healthy one gets exactly its tokens."""
+    g = gen(len(cu) + cu[1])
+    lens = [40, 100]  # rows after the append, histories before it
+    _, cache = paged_case(g, 4, 2, 64, 16, lens, "bf16")
+    k0, v0 = cache.k.clone(), cache.v.clone()
+    k, v, q = normal(g, 40, 2, 64), normal(g, 40, 2, 64), normal(g, 40, 4, 64)
+    gpu_ctx.kv_append(cache, k, v, ints(lens), cu_new=ints(cu), q=q)
+    reported(gpu_ctx, "offsets")
+    if healthy is not None:
+        for s in healthy:
+            p = torch.arange(lens[s] - (cu[s + 1] - cu[s]), lens[s], device="cuda")
+            at, off = cache.block_table[s][p // 16].long(), p % 16
+            k0[at, :, off], v0[at, :, off] = k[cu[s]:cu[s + 1]], v[cu[s]:cu[s + 1]]
+        assert torch.equal(cache.k, k0) and torch.equal(cache.v, v0)
+    gpu_ctx.kv_append(cache, k, v, ints(lens), cu_new=ints([0, 20, 40]))
+    gpu_ctx.sync()  # the context goes on
+    for s in range(2):
+        ck, cv = gathered(cache, s, lens[s])
+        assert torch.equal(ck[-20:], k[20 * s:20 * s + 20]) and torch.equal(cv[-20:], v[20 * s:20 * s + 20])
+
+
+def test_append_reports_one_falling_pair_among_many_sequences(gpu_ctx):
+    """A pair that no token's own sequence shows, first, last and far from both."""
+    n_seqs = 5000
+    table = torch.arange(n_seqs, device="cuda", dtype=torch.int32)[:, None].contiguous()
+    kc, vc = (torch.zeros(n_seqs, 1, 4, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    g = gen(2)
+    for tokens in (1, 700):
+        k, v = normal(g, tokens, 1, 64, dtype="f16"), normal(g, tokens, 1, 64, dtype="f16")
+        cu = torch.zeros(n_seqs + 1, dtype=torch.int32, device="cuda")
+        cu[n_seqs // 2:] = tokens
+        lens = torch.full((n_seqs,), 4, dtype=torch.int32, device="cuda")
+        for at in (1, n_seqs // 4, n_seqs // 2 - 1):  # a rise and a fall among empty sequences
+            bad = cu.clone()
+            bad[at] = 1 if tokens == 1 else 3
+            bad[n_seqs // 2:] = tokens
+            if at + 1 == n_seqs // 2:
+                bad[at] = tokens + 5
+            gpu_ctx.kv_append(PagedKv(kc, vc, table), k, v, lens, cu_new=bad)
+            reported(gpu_ctx, "offsets")
+        # the pad rows behind the last sequence are no fault
+        cu[n_seqs // 2:] = tokens // 2
+        gpu_ctx.kv_append(PagedKv(kc, vc, table), k, v, lens, cu_new=cu)
+        gpu_ctx.sync()
