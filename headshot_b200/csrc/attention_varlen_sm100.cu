@@ -60,6 +60,8 @@
 //   four MMAs per election (1,214 / 781 to 801)
 #include <cuda.h>
 
+#include <float.h>
+
 #include <algorithm>
 
 #include "hs_internal.h"
@@ -235,9 +237,10 @@ __device__ __forceinline__ uint32_t wg_tiles(const Args& a, const Item& it, int 
   return keys > 0 ? static_cast<uint32_t>(keys + Shape<D>::kBN - 1) / Shape<D>::kBN : 0u;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// The largest of three; NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -334,8 +337,8 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
       bool need = false;
       float m4[4] = {u2f(s[0]), u2f(s[1]), u2f(s[2]), u2f(s[3])};
 #pragma unroll
-      for (int i = 4; i < kBN; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], u2f(s[i]), u2f(s[i + 1]));
-      const float m_tile = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * c;
+      for (int i = 4; i < kBN; i += 2) m4[(i >> 1) & 3] = max3_nan(m4[(i >> 1) & 3], u2f(s[i]), u2f(s[i + 1]));
+      const float m_tile = max3_nan(max3_nan(m4[0], m4[0], m4[1]), m4[2], m4[3]) * c;
       if (j == 0) {
         m_run = m_tile;
       } else if (m_tile > m_run + kRescaleThreshold) {
@@ -344,6 +347,10 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
         l *= factor;
         need = true;
       }
+      // A NaN score (or one past f32) makes the row's sum, and so its output, NaN
+      // through its maximum: the FMA pipe's exponential alone would clamp it to a
+      // weight of zero, and the key would be gone without a trace.
+      l = fmaf(max3_nan(m_tile, m_tile, -FLT_MAX), 0.f, l);
       // A row that sees no key has m_run = -inf and turns into NaN here: its
       // output is set to zero below, and no other row reads it.
       // The exponents s c - m are one fused step each; the rounding of m = max c

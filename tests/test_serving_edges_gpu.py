@@ -4,6 +4,8 @@ a tile, scores of any size, equal bits whatever the block table's width, a works
 for the next call, refusals by the library itself.  Tolerances as in test_serving_gpu.py."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -78,3 +80,42 @@ def test_append_reports_one_falling_pair_among_many_sequences(gpu_ctx):
         cu[n_seqs // 2:] = tokens // 2
         gpu_ctx.kv_append(PagedKv(kc, vc, table), k, v, lens, cu_new=cu)
         gpu_ctx.sync()
+
+
+# --------------------------------------------------------------- NaN keys --
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_nan_key_reaches_every_row_that_sees_it(gpu_ctx, dtype, d):
+    """A NaN score makes its row NaN, whichever position of a key tile it has, and no other row."""
+    g = gen(d)
+    n = 200  # two and more tiles of 64 and 96 keys: every position of a first and of a later tile
+    q = normal(g, n, 2, d, dtype=dtype)  # sequence p: one query, n keys, key p is not a number
+    k, v = normal(g, n, n, 1, d, dtype=dtype), normal(g, n * n, 1, d, dtype=dtype)
+    p = torch.arange(n, device="cuda")
+    k[p, p, 0, p % d] = math.nan
+    out = gpu_ctx.attention_varlen(q, k.view(n * n, 1, d), v, offsets([1] * n), cu_k=offsets([n] * n), causal=False)
+    gpu_ctx.sync()
+    assert out.isnan().all()
+
+    kc = normal(g, n, 1, d, dtype=dtype)
+    clean = gpu_ctx.attention_varlen(q, kc, v[:n], offsets([n]))
+    for at in (0, 63, 64, 95, 96, 127, 150, 191, 192, 199):
+        kn = kc.clone()
+        kn[at, 0, 3] = math.nan
+        out = gpu_ctx.attention_varlen(q, kn, v[:n], offsets([n]))
+        gpu_ctx.sync()
+        assert out[at:].isnan().all() and torch.equal(out[:at], clean[:at])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_nan_key_in_the_cache(gpu_ctx, d):
+    n = 150
+    g = gen(d + 1)
+    q, cache = paged_case(g, 4, 2, d, 16, [n] * n, "bf16")
+    p = torch.arange(n, device="cuda")
+    cache.k[cache.block_table[p, p // 16].long(), 0, p % 16, 5] = math.nan  # key p of sequence p, first key head
+    out = gpu_ctx.attention_paged(q, cache, ints([n] * n))
+    gpu_ctx.sync()
+    assert out[:, :2].isnan().all() and torch.isfinite(out[:, 2:]).all()
