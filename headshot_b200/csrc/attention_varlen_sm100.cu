@@ -49,7 +49,8 @@
 // Steps kept, on these two in TFLOP/s: 1,215 / 790 -> tested waits 1,240 / 798
 // -> the next K/V tile awaited before P 1,278 / 825 -> P stored 16 columns at
 // a time 1,312 / 830 -> the FMA pipe's share last of each 16 pairs, masked
-// weights exactly zero 1,329 / 837.  Built and not kept, against the 1,215 / 790:
+// weights exactly zero 1,329 / 837 -> exponents of score differences, right for any
+// finite score, 1,290 / 834.  Built and not kept, against the 1,215 / 790:
 //   head_dim 128 with 128-key tiles and one score buffer (1,079; with one MMA
 //     warp for both warpgroups 1,170, without splitting P's hand-over 1,251 in
 //     a burst, 1,052 against 1,141 at the power cap)
@@ -286,6 +287,7 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
   const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
   const uint32_t tO = tmem + lane_base + S::col_o(wg);
   const float c = a.scale_log2;
+  const float threshold = fminf(kRescaleThreshold / c, 1e30f);  // of scores before the scale
   // The row's token within the tile and head within the group.
   const uint32_t tok = row / a.group, head = row - tok * a.group;
   const bool in_tile = tok < a.tile_tokens;
@@ -333,37 +335,30 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
         for (int i = 0; i < kBN; ++i)
           if (i > left) s[i] = __float_as_uint(-INFINITY);
       }
-      float factor = 1.f;
       bool need = false;
       float m4[4] = {u2f(s[0]), u2f(s[1]), u2f(s[2]), u2f(s[3])};
 #pragma unroll
       for (int i = 4; i < kBN; i += 2) m4[(i >> 1) & 3] = max3_nan(m4[(i >> 1) & 3], u2f(s[i]), u2f(s[i + 1]));
-      const float m_tile = max3_nan(max3_nan(m4[0], m4[0], m4[1]), m4[2], m4[3]) * c;
-      if (j == 0) {
+      const float m_tile = max3_nan(max3_nan(m4[0], m4[0], m4[1]), m4[2], m4[3]);
+      const float m_old = m_run;
+      if (j == 0 || m_tile > m_run + threshold) {
         m_run = m_tile;
-      } else if (m_tile > m_run + kRescaleThreshold) {
-        factor = ex2_approx(m_run - m_tile);
-        m_run = m_tile;
-        l *= factor;
-        need = true;
+        need = j > 0;
       }
-      // A NaN score (or one past f32) makes the row's sum, and so its output, NaN
-      // through its maximum: the FMA pipe's exponential alone would clamp it to a
-      // weight of zero, and the key would be gone without a trace.
-      l = fmaf(max3_nan(m_tile, m_tile, -FLT_MAX), 0.f, l);
       // A row that sees no key has m_run = -inf and turns into NaN here: its
       // output is set to zero below, and no other row reads it.
-      // The exponents s c - m are one fused step each; the rounding of m = max c
-      // is common to a row and cancels in O / l as long as it stays within the
-      // type's binades, for scores to 2^26.  (Differences first, for any score: a
-      // branch here costs 13 %.)
+      // The exponents are (s - m) c, right for any finite score.  (s c - m c in one
+      // fused step is 1.3 to 2.6 % faster on long prompts, but m c rounds away
+      // binades from 2^26 on; telling such rows apart costs more than the second
+      // step: 16 % by a branch here, 5 % by a flag that only reports them.)
       const float neg_m = -m_run;
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
       uint32_t pk[S::kPairs];
 #pragma unroll
       for (int i = 0; i < S::kPairs; ++i) {
         float x0, x1, p0, p1;
-        fma2(x0, x1, u2f(s[2 * i]), u2f(s[2 * i + 1]), c, c, neg_m, neg_m);
+        add2(x0, x1, u2f(s[2 * i]), u2f(s[2 * i + 1]), neg_m, neg_m);
+        mul2(x0, x1, x0, x1, c, c);
         if ((i & 15) >= 16 - S::kEmuPer16) {
           exp2_poly2(x0, x1, p0, p1);
         } else {
@@ -374,7 +369,11 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
         add2(acc[2 * (i & 1)], acc[2 * (i & 1) + 1], acc[2 * (i & 1)], acc[2 * (i & 1) + 1], p0, p1);
         if (i % 16 == 15) tmem_st16(tS + i - 15, pk + i - 15);
       }
-      l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      float sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      // A NaN score (or one past f32) makes the row's sum, and so its output, NaN
+      // through its maximum: the FMA pipe's exponential alone would clamp it to a
+      // weight of zero, and the key would be gone without a trace.
+      sum = fmaf(max3_nan(m_tile, m_tile, -FLT_MAX), 0.f, sum);
       // O rescale (rare), once PV(j-1) has landed: committed with S(j+1) when
       // that tile exists, else (j = n-1) as the item's first PV-only batch.
       if (__any_sync(0xffffffffu, need)) {
@@ -384,6 +383,8 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
                                                 kSiteODone, a.timeout_ns);
         if (!ok) return;
         tc_fence_after();
+        const float factor = need ? ex2_approx((m_old - m_run) * c) : 1.f;
+        l *= factor;
 #pragma unroll
         for (int h = 0; h < D / 16; ++h) {
           uint32_t o[16];
@@ -394,6 +395,7 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
           tmem_st16(tO + 16 * h, o);
         }
       }
+      l += sum;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();

@@ -276,8 +276,8 @@ HS_API hs_status hs_kv_append(hs_ctx* ctx, const void* q, const void* k, const v
  * sees every key); else all Lk.  A query that sees none is zero.  out
  * (total_q, Hq*D); rows from cu_q[n_seqs] on are left as they were.  Keys
  * and values past a sequence's end never take part, whatever they hold; the
- * values of a sequence's own keys must be finite, and scores (q.k scale)
- * within +-2^26.  Hq / Hkv <= 128.
+ * values of a sequence's own keys and the scores (q.k in f32) must be
+ * finite: a NaN key makes the queries that see it NaN.  Hq / Hkv <= 128.
  * scale <= 0 selects 1/sqrt(D). */
 HS_API hs_status hs_attention_varlen(hs_ctx* ctx, const void* q, const void* k, const void* v, void* out,
                                      uint64_t q_stride, uint64_t k_stride, uint64_t v_stride, const int* cu_q,

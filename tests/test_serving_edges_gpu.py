@@ -11,7 +11,7 @@ import torch
 
 from headshot_b200._lib import HS_ERR_INVALID, HsError
 from headshot_b200.engine import PagedKv
-from test_serving_gpu import gathered, gen, ints, normal, offsets, paged_case
+from test_serving_gpu import check_attention, gathered, gen, ints, normal, offsets, paged_case
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +119,48 @@ def test_one_nan_key_in_the_cache(gpu_ctx, d):
     out = gpu_ctx.attention_paged(q, cache, ints([n] * n))
     gpu_ctx.sync()
     assert out[:, :2].isnan().all() and torch.isfinite(out[:, 2:]).all()
+
+
+# ------------------------------------------------------------ score range --
+
+
+@pytest.mark.parametrize("dtype,size", [("bf16", 2e3), ("bf16", 1e5), ("bf16", 1e9), ("bf16", 1e15), ("f16", 2e3), ("f16", 6e4)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_scores_of_any_size(gpu_ctx, dtype, size, d):
+    """Each row belongs to its largest score, which the inputs set apart from the others by far: score
+    d size^2, the next one 2 size^2 less at least."""
+    g = gen(18)
+    n = 130
+    sign = torch.where(torch.rand(n, 1, d, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    k = (sign * size).to(torch.bfloat16 if dtype == "bf16" else torch.float16)
+    q = k.flip(0)
+    v = normal(g, n, 1, d, dtype=dtype)
+    out = gpu_ctx.attention_varlen(q, k, v, offsets([n]), causal=False)
+    gpu_ctx.sync()
+    check_attention(out, v.flip(0).double(), v.flip(0).double().abs(), n, dtype, v.abs().max().item())
+
+
+@pytest.mark.parametrize("dtype,size", [("bf16", 1.0), ("bf16", 2.0 ** 10), ("bf16", 2.0 ** 20), ("bf16", 2.0 ** 60), ("f16", 2.0 ** 10), ("f16", 2.0 ** 15)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("step", [1, -1])
+def test_prompt_maximum_that_moves_through_every_size(gpu_ctx, dtype, size, d, step):
+    """Key j scores d size (j - 150) before the scale, rising or falling: with at least d / sqrt(d) = 8
+    between neighbours a row is its largest key's value but for weights of e^-8 and less, which the
+    reference counts; sizes run from small scores to ones whose spacing in f32 is many binades."""
+    g = gen(19)
+    n = 300
+    t = torch.bfloat16 if dtype == "bf16" else torch.float16
+    j = torch.arange(n, device="cuda") - 150
+    j = torch.where(j.abs() > 128, j.sign() * 128, j)  # whole in bf16 too; ties at both ends share their weight
+    k = (j * step).to(t)[:, None, None].expand(n, 1, d).contiguous()
+    q = torch.full((n, 2, d), size, dtype=t, device="cuda")
+    v = normal(g, n, 1, d, dtype=dtype)
+    out = gpu_ctx.attention_varlen(q, k, v, offsets([n]))
+    gpu_ctx.sync()
+    # every product and partial sum is whole times size, so scores are exact in f32 and in f64
+    s = torch.outer(torch.ones(n, device="cuda", dtype=torch.float64), j.double() * step) * (d * size * d ** -0.5)
+    s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(1), -math.inf)
+    w = torch.softmax(s, -1)
+    ref, mass = w @ v[:, 0].double(), w @ v[:, 0].double().abs()
+    for h in range(2):
+        check_attention(out[:, h], ref, mass, n, dtype, v.abs().max().item())
