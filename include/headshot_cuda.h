@@ -294,7 +294,8 @@ HS_API hs_status hs_attention_paged_workspace(hs_ctx* ctx, size_t* bytes);
  * q_stride attends to the first kv_lens[s] cached tokens; out (n_seqs,
  * Hq*D).  kv_lens[s] <= 0 gives a zero row.  The cache's length is split over
  * the GPU and joined within the call, in an order that depends on the
- * lengths only, so equal calls give equal bits.  scale as above. */
+ * lengths, the heads and the GPU's number of SMs only, so equal calls give
+ * equal bits, whatever the block table's width.  scale as above. */
 HS_API hs_status hs_attention_paged(hs_ctx* ctx, const void* q, void* out, const void* k_cache, const void* v_cache,
                                     const int* block_table, const int* kv_lens, uint64_t q_stride, uint32_t n_seqs,
                                     uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size,

@@ -11,7 +11,7 @@ import torch
 
 from headshot_b200._lib import HS_ERR_INVALID, HsError
 from headshot_b200.engine import PagedKv
-from test_serving_gpu import check_attention, gathered, gen, ints, normal, offsets, paged_case
+from test_serving_gpu import check_attention, gathered, gen, ints, normal, offsets, paged_case, paged_check
 
 pytestmark = pytest.mark.gpu
 
@@ -164,3 +164,22 @@ def test_prompt_maximum_that_moves_through_every_size(gpu_ctx, dtype, size, d, s
     ref, mass = w @ v[:, 0].double(), w @ v[:, 0].double().abs()
     for h in range(2):
         check_attention(out[:, h], ref, mass, n, dtype, v.abs().max().item())
+
+
+# ------------------------------------------------------------ paged split --
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (16, 16, 64), (4, 1, 128)])
+@pytest.mark.parametrize("lens", [[8191], [5000, 17, 700, 0, 2300]])
+def test_paged_bits_do_not_depend_on_the_table_width(gpu_ctx, hq, hkv, d, lens):
+    """The split of the keys over the GPU follows the lengths, not the room that the table has."""
+    q, cache = paged_case(gen(50), hq, hkv, d, 16, lens, "bf16")
+    outs = []
+    for wide in (0, 3, 700, 20000):
+        table = torch.full((len(lens), cache.block_table.shape[1] + wide), -1, dtype=torch.int32, device="cuda")
+        table[:, :cache.block_table.shape[1]] = cache.block_table
+        outs.append(gpu_ctx.attention_paged(q, PagedKv(cache.k, cache.v, table), ints(lens)))
+    gpu_ctx.sync()
+    for x in outs[1:]:
+        assert torch.equal(outs[0], x)
+    paged_check(outs[0], q, cache, lens, "bf16")
