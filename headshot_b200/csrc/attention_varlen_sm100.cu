@@ -860,6 +860,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 8) {
     regs_inc<kSoftmaxRegs>();
     softmax_role<E, D>(a, ctl, tmem, warp, lane);
+    // A role that gave up in the middle of a tile may have stores to TMEM in
+    // flight; they land before it is freed.
+    __syncwarp();
+    tmem_wait_st();
   } else {
     regs_dec<kControlRegs>();
     if (warp == kProducerWarp)

@@ -9,8 +9,8 @@ import math
 import pytest
 import torch
 
-from headshot_b200._lib import HS_ERR_INVALID, HsError
-from headshot_b200.engine import PagedKv
+from headshot_b200._lib import HS_ERR_INVALID, HS_ERR_TIMEOUT, HsError
+from headshot_b200.engine import GpuContext, PagedKv
 from test_serving_gpu import check_attention, gathered, gen, ints, normal, offsets, paged_case, paged_check
 
 pytestmark = pytest.mark.gpu
@@ -164,6 +164,34 @@ def test_prompt_maximum_that_moves_through_every_size(gpu_ctx, dtype, size, d, s
     ref, mass = w @ v[:, 0].double(), w @ v[:, 0].double().abs()
     for h in range(2):
         check_attention(out[:, h], ref, mass, n, dtype, v.abs().max().item())
+
+
+# -------------------------------------------------------------- time-outs --
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_gives_up_while_it_rescales(d):
+    """Wait bound 0 on scores whose maximum moves with every tile: a row that waits to rescale its
+    output gives up too, and the next call with the usual bound is right."""
+    ctx = GpuContext(0)
+    g = gen(60)
+    n = 1500
+    q = torch.full((n, 4, d), 2.0, dtype=torch.bfloat16, device="cuda")
+    k = (torch.arange(n, device="cuda") / 8).to(torch.bfloat16)[:, None, None].expand(n, 2, d).contiguous()
+    v = normal(g, n, 2, d)
+    good = ctx.attention_varlen(q, k, v, offsets([n]))
+    ctx.sync()
+    for _ in range(5):
+        ctx.set_wait_timeout_ms(0)
+        ctx.attention_varlen(q, k, v, offsets([n]))
+        with pytest.raises(HsError) as e:
+            ctx.sync()
+        assert e.value.status == HS_ERR_TIMEOUT
+        ctx.set_wait_timeout_ms(2000)
+        again = ctx.attention_varlen(q, k, v, offsets([n]))
+        ctx.sync()
+        assert torch.equal(good, again)
+    ctx.close()
 
 
 # ------------------------------------------------------------ paged split --
