@@ -10,8 +10,8 @@ import pytest
 import torch
 
 from headshot_b200._lib import HS_ERR_INVALID, HS_ERR_TIMEOUT, HsError
-from headshot_b200.engine import GpuContext, PagedKv
-from test_serving_gpu import check_attention, gathered, gen, ints, normal, offsets, paged_case, paged_check
+from headshot_b200.engine import GpuContext, PagedKv, Rope
+from test_serving_gpu import check_attention, gathered, gen, ints, normal, offsets, paged_case, paged_check, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -82,6 +82,28 @@ def test_append_reports_one_falling_pair_among_many_sequences(gpu_ctx):
         gpu_ctx.sync()
 
 
+def test_append_bad_page_leaves_the_rest_exact(gpu_ctx):
+    """One sequence's bad page, length or rotation row: the others' tokens are written exactly, and
+    nothing else of either cache changes."""
+    g = gen(24)
+    k, v = normal(g, 3, 2, 64), normal(g, 3, 2, 64)
+    _, cache = paged_case(g, 4, 2, 64, 16, [40, 40, 40], "bf16")
+    for what, lens, rope, word in (("page", [40, 40, 40], None, "page"), ("length", [40, 49, 40], None, "length"),
+                                   # rows below the prefix of 30 pass through; position 39 asks for row 9 of 9
+                                   ("row", [30, 40, 30], Rope(*tables(9, 64, 2), 30), "rotation")):
+        kc, vc, table = cache.k.clone(), cache.v.clone(), cache.block_table.clone()
+        if what == "page":
+            table[1, 2] = kc.shape[0]
+        want_k, want_v = kc.clone(), vc.clone()
+        for s in (0, 2):
+            p = lens[s] - 1
+            at = table[s, p // 16].long()
+            want_k[at, :, p % 16], want_v[at, :, p % 16] = k[s], v[s]
+        gpu_ctx.kv_append(PagedKv(kc, vc, table), k, v, ints(lens), rope=rope)
+        reported(gpu_ctx, word)
+        assert torch.equal(kc, want_k) and torch.equal(vc, want_v)
+
+
 # --------------------------------------------------------------- NaN keys --
 
 
@@ -119,6 +141,23 @@ def test_one_nan_key_in_the_cache(gpu_ctx, d):
     out = gpu_ctx.attention_paged(q, cache, ints([n] * n))
     gpu_ctx.sync()
     assert out[:, :2].isnan().all() and torch.isfinite(out[:, 2:]).all()
+
+
+# ------------------------------------------------------------ packed rows --
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_offsets_into_a_larger_pack(gpu_ctx, causal):
+    """A slice of a pack's offsets attends for its sequences alone; rows before and behind stay."""
+    g = gen(31)
+    lens = [30, 130, 1, 70, 9]
+    q, k, v = normal(g, 240, 4, 64), normal(g, 240, 2, 64), normal(g, 240, 2, 64)
+    cu = offsets(lens)
+    whole = gpu_ctx.attention_varlen(q, k, v, cu, causal=causal)
+    out = torch.full_like(q, 7)
+    gpu_ctx.attention_varlen(q, k, v, cu[1:4].contiguous(), causal=causal, out=out)
+    gpu_ctx.sync()
+    assert (out[:30] == 7).all() and torch.equal(out[30:161], whole[30:161]) and (out[161:] == 7).all()
 
 
 # ------------------------------------------------------------ score range --
@@ -211,3 +250,66 @@ def test_paged_bits_do_not_depend_on_the_table_width(gpu_ctx, hq, hkv, d, lens):
     for x in outs[1:]:
         assert torch.equal(outs[0], x)
     paged_check(outs[0], q, cache, lens, "bf16")
+
+
+def test_paged_leaves_its_workspace_ready(gpu_ctx):
+    """The counters (the first 4 KiB) are zero again after every call, so the next one may be of any shape."""
+    ws = gpu_ctx.paged_workspace()
+    for seqs, longest, hq, hkv, d in ((1, 30000, 8, 8, 128), (300, 40, 4, 2, 64), (37, 3001, 8, 8, 64), (2, 20001, 48, 1, 128),
+                                      (700, 9, 2, 1, 128), (1, 9000, 2, 1, 64)):
+        g = gen(seqs)
+        lens = torch.randint(0, longest + 1, (seqs,), generator=g, device="cuda").tolist()
+        lens[-1] = longest
+        q, cache = paged_case(g, hq, hkv, d, 16, lens, "bf16")
+        outs = []
+        for _ in range(2):
+            outs.append(gpu_ctx.attention_paged(q, cache, ints(lens), workspace=ws))
+            gpu_ctx.sync()
+            assert (ws[:4096] == 0).all()
+        assert torch.equal(*outs)
+        paged_check(outs[0], q, cache, lens, "bf16")
+    assert (ws[4096:] != 0).any()  # the calls did cut sequences
+
+
+# --------------------------------------------------------------- refusals --
+
+
+def test_the_library_refuses_by_itself(gpu_ctx):
+    """Through the C ABI, past the Python checks: each call returns a status and launches nothing."""
+    L, h = gpu_ctx._L, gpu_ctx._h
+    x = torch.zeros(1 << 16, dtype=torch.bfloat16, device="cuda")
+    i = torch.zeros(64, dtype=torch.int32, device="cuda")
+    f = torch.zeros(1 << 12, dtype=torch.float32, device="cuda")
+    ws = gpu_ctx.paged_workspace()
+    X, I, F, bf16 = x.data_ptr(), i.data_ptr(), f.data_ptr(), 2
+
+    def append(q=X, k=X, v=X, qo=X + 32768, ko=0, kc=X, vc=X, table=I, lens=I, cu=0, qs=0, ks=0, vs=0, n=2, seqs=2, hq=4,
+               hkv=2, d=64, pages=4, page=16, most=2, dt=bf16, sin=0, cos=0, rows=0, prefix=0, tpf=0):
+        return L.hs_kv_append(h, q, k, v, qo, ko, kc, vc, table, lens, cu, qs, ks, vs, n, seqs, hq, hkv, d, pages, page, most,
+                              dt, sin, cos, rows, prefix, tpf)
+
+    def varlen(q=X, k=X, v=X, out=X, qs=0, ks=0, vs=0, cq=I, ck=0, tq=2, tk=2, seqs=1, hq=4, hkv=2, d=64, causal=1, dt=bf16):
+        return L.hs_attention_varlen(h, q, k, v, out, qs, ks, vs, cq, ck, tq, tk, seqs, hq, hkv, d, causal, dt, 0.0)
+
+    def paged(q=X, out=X, kc=X, vc=X, table=I, lens=I, qs=0, seqs=2, hq=4, hkv=2, d=64, pages=4, page=16, most=2, dt=bf16,
+              w=ws.data_ptr(), nb=ws.nbytes):
+        return L.hs_attention_paged(h, q, out, kc, vc, table, lens, qs, seqs, hq, hkv, d, pages, page, most, dt, 0.0, w, nb)
+
+    bad = [
+        *(append(**{a: 0}) for a in ("k", "v", "qo", "kc", "vc", "table", "lens", "hkv", "page", "q")),
+        *(append(**{a: X + 2}) for a in ("q", "k", "v", "qo", "ko", "kc", "vc")), append(table=I + 2), append(cu=I + 1),
+        append(n=3), append(hq=5), append(hq=1026), append(hq=4096, hkv=2048), append(d=96), append(dt=0), append(dt=9),
+        append(qs=100), append(ks=129), append(vs=64), append(sin=F), append(sin=F, cos=F + 4), append(pages=2 ** 31),
+        append(page=2 ** 16, most=2 ** 16), append(sin=F, cos=F, rows=18, prefix=5, tpf=24),
+        append(sin=F, cos=F, rows=18, prefix=25, tpf=24), append(qo=X, qs=512), append(ko=X, ks=256),
+        append(n=2 ** 31, cu=I), append(seqs=2 ** 31 - 1, cu=I),
+        *(varlen(**{a: 0}) for a in ("q", "k", "v", "out", "cq", "hkv")), *(varlen(**{a: X + 8}) for a in ("q", "k", "v", "out")),
+        varlen(cq=I + 2), varlen(tk=3), varlen(hq=129 * 2), varlen(hq=3), varlen(d=32), varlen(dt=0), varlen(qs=250),
+        varlen(ks=64), varlen(vs=132), varlen(tq=2 ** 31, tk=2 ** 31), varlen(seqs=2 ** 31 - 1),
+        varlen(qs=2 ** 33),
+        *(paged(**{a: 0}) for a in ("q", "out", "kc", "vc", "table", "lens", "hkv", "page", "w")),
+        *(paged(**{a: X + 8}) for a in ("q", "out", "kc", "vc")), paged(w=ws.data_ptr() + 8), paged(nb=ws.nbytes - 1),
+        paged(hq=3), paged(d=96), paged(dt=0), paged(qs=8), paged(seqs=2 ** 30), paged(pages=2 ** 32 - 1),
+    ]
+    assert all(s != 0 for s in bad), [n for n, s in enumerate(bad) if s == 0]
+    gpu_ctx.sync()
