@@ -44,6 +44,22 @@ hs_status fix_stride(const char* name, const char* which, uint32_t heads, uint32
   return HS_OK;
 }
 
+// Head vectors of n tokens, 16-bit elements.
+struct Rows {
+  const void* at;
+  uint64_t n, stride, row;
+  uint64_t begin() const { return reinterpret_cast<uintptr_t>(at); }
+  uint64_t end() const { return at && n && row ? begin() + 2 * ((n - 1) * stride + row) : begin(); }
+};
+bool overlap(const Rows& a, const Rows& b) {
+  return a.begin() < a.end() && b.begin() < b.end() && a.begin() < b.end() && b.begin() < a.end();
+}
+// Whether `out` may be written while `in` is read: apart, or the same rows,
+// since each of them is read whole before its own place is written.
+bool apart_or_same(const Rows& out, const Rows& in) {
+  return !overlap(out, in) || (out.at == in.at && (in.stride == out.stride || in.n == 1) && in.row == out.row);
+}
+
 hs_status check_cache(const char* name, const void* k_cache, const void* v_cache, const int* block_table,
                       const int* kv_lens, uint32_t n_pages, uint32_t page_size, uint32_t max_pages) {
   if (!k_cache || !v_cache || !block_table || !kv_lens) return invalid(name, "null cache pointer");
@@ -106,10 +122,14 @@ hs_status hs_kv_append(hs_ctx* ctx, const void* q, const void* k, const void* v,
     if (q && (r = fix_stride(name, "q", Hq, D, &q_stride)) != HS_OK) return r;
     if ((r = fix_stride(name, "k", Hkv, D, &k_stride)) != HS_OK) return r;
     if ((r = fix_stride(name, "v", Hkv, D, &v_stride)) != HS_OK) return r;
-    if (q == q_out && q && q_stride != static_cast<uint64_t>(Hq) * D)
-      return invalid(name, "in place q needs contiguous tokens");
-    if (k == k_out && k_stride != static_cast<uint64_t>(Hkv) * D)
-      return invalid(name, "in place k needs contiguous tokens");
+    const uint64_t q_row = static_cast<uint64_t>(Hq) * D, k_row = static_cast<uint64_t>(Hkv) * D;
+    const Rows rq{q, n_tokens, q_stride, q_row}, rk{k, n_tokens, k_stride, k_row}, rv{v, n_tokens, v_stride, k_row};
+    const Rows rqo{q_out, n_tokens, q_row, q_row}, rko{k_out, n_tokens, k_row, k_row};
+    if (q && !apart_or_same(rqo, rq)) return invalid(name, "in place q needs contiguous tokens");
+    if (k_out && !apart_or_same(rko, rk)) return invalid(name, "in place k needs contiguous tokens");
+    if ((q && (overlap(rqo, rk) || overlap(rqo, rv))) ||
+        (k_out && (overlap(rko, rv) || (q && (overlap(rko, rq) || overlap(rko, rqo))))))
+      return invalid(name, "q_out and k_out must not overlap other tensors");
     KvAppend a;
     a.q = q;
     a.k = k;
@@ -155,6 +175,11 @@ hs_status hs_attention_varlen(hs_ctx* ctx, const void* q, const void* k, const v
     if ((r = fix_stride(name, "q", Hq, D, &q_stride)) != HS_OK) return r;
     if ((r = fix_stride(name, "k", Hkv, D, &k_stride)) != HS_OK) return r;
     if ((r = fix_stride(name, "v", Hkv, D, &v_stride)) != HS_OK) return r;
+    const uint64_t q_row = static_cast<uint64_t>(Hq) * D, k_row = static_cast<uint64_t>(Hkv) * D;
+    const Rows ro{out, total_q, q_row, q_row};
+    if (!apart_or_same(ro, Rows{q, total_q, q_stride, q_row}) || overlap(ro, Rows{k, total_k, k_stride, k_row}) ||
+        overlap(ro, Rows{v, total_k, v_stride, k_row}))
+      return invalid(name, "out must not overlap k or v, and q only as the same contiguous rows");
     if (!(scale > 0.f) || !isfinite(scale)) scale = 1.0f / sqrtf(static_cast<float>(D));
     VarlenIO io;
     io.q = q;
@@ -211,6 +236,9 @@ hs_status hs_attention_paged(hs_ctx* ctx, const void* q, void* out, const void* 
     r = check_cache(name, k_cache, v_cache, block_table, kv_lens, n_pages, page_size, max_pages);
     if (r != HS_OK) return r;
     if ((r = fix_stride(name, "q", Hq, D, &q_stride)) != HS_OK) return r;
+    const uint64_t q_row = static_cast<uint64_t>(Hq) * D;
+    if (!apart_or_same(Rows{out, n_seqs, q_row, q_row}, Rows{q, n_seqs, q_stride, q_row}))
+      return invalid(name, "in place q needs contiguous tokens");
     if (!(scale > 0.f) || !isfinite(scale)) scale = 1.0f / sqrtf(static_cast<float>(D));
     DeviceGuard guard(ctx->device);
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < attention_paged_workspace_bytes())

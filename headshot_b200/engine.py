@@ -297,7 +297,8 @@ class GpuContext:
         """Attention of packed sequences: q (tokens, heads, D), k and v (tokens, kv_heads, D); tokens
         [cu[s], cu[s+1]) are sequence s (cu_k: other lengths for k and v).  Causal masks align to the
         end: the last query sees every key.  Returns (tokens, heads, D); queries that see no key are
-        zero, rows past cu_q[-1] are left as they were (uninitialised where `out` is allocated here).
+        zero, rows before cu_q[0] and past cu_q[-1] are left as they were (uninitialised where `out` is
+        allocated here); `out` may be q where that is contiguous, and overlaps neither k nor v.
         Values and scores (q.k in f32) must be finite; a NaN key makes the queries that see it NaN."""
         t, hq, d, qs = self._check_rows(q, "q")
         tk, hkv, dk, ks = self._check_rows(k, "k")

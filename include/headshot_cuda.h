@@ -261,7 +261,7 @@ HS_API hs_status hs_attn_merge(hs_ctx* ctx, const void* x, void* out, uint32_t S
  * q (may be NULL, then q_out is NULL): the tokens' queries, rotated into
  * q_out (n_tokens, Hq, D).  k_out (may be NULL): the rotated keys once more,
  * (n_tokens, Hkv, D), for hs_attention_varlen.  q_out may be q and k_out may
- * be k where those are contiguous. */
+ * be k where those are contiguous; they overlap nothing else. */
 HS_API hs_status hs_kv_append(hs_ctx* ctx, const void* q, const void* k, const void* v, void* q_out, void* k_out,
                               void* k_cache, void* v_cache, const int* block_table, const int* kv_lens,
                               const int* cu_new, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
@@ -274,7 +274,8 @@ HS_API hs_status hs_kv_append(hs_ctx* ctx, const void* q, const void* k, const v
  * tokens [cu_k[s], cu_k[s+1]) of k and v (cu_k NULL: cu_q, total_k ==
  * total_q).  causal: query i of Lq sees keys j <= i + Lk - Lq (the last query
  * sees every key); else all Lk.  A query that sees none is zero.  out
- * (total_q, Hq*D); rows from cu_q[n_seqs] on are left as they were.  Keys
+ * (total_q, Hq*D) may be q where that is contiguous and overlaps neither k
+ * nor v; rows before cu_q[0] and from cu_q[n_seqs] on are left as they were.  Keys
  * and values past a sequence's end never take part, whatever they hold; the
  * values of a sequence's own keys and the scores (q.k in f32) must be
  * finite: a NaN key makes the queries that see it NaN.  Hq / Hkv <= 128.
@@ -292,7 +293,8 @@ HS_API hs_status hs_attention_paged_workspace(hs_ctx* ctx, size_t* bytes);
 
 /* One new token per sequence against its cache: q (n_seqs, Hq, D) at
  * q_stride attends to the first kv_lens[s] cached tokens; out (n_seqs,
- * Hq*D).  kv_lens[s] <= 0 gives a zero row.  The cache's length is split over
+ * Hq*D), which may be q where that is contiguous.  kv_lens[s] <= 0 gives a
+ * zero row.  The cache's length is split over
  * the GPU and joined within the call, in an order that depends on the
  * lengths, the heads and the GPU's number of SMs only, so equal calls give
  * equal bits, whatever the block table's width.  scale as above. */

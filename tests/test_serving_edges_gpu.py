@@ -313,3 +313,48 @@ def test_the_library_refuses_by_itself(gpu_ctx):
     ]
     assert all(s != 0 for s in bad), [n for n, s in enumerate(bad) if s == 0]
     gpu_ctx.sync()
+
+
+def test_outputs_in_place_and_overlapping(gpu_ctx):
+    """The queries' own contiguous rows may take the output; any other overlap with an input is refused."""
+    g = gen(70)
+    lens = [300, 45, 1, 129]
+    n = sum(lens)
+    for hq, hkv, d in ((4, 4, 64), (6, 2, 128), (10, 2, 64)):
+        q, k, v = normal(g, n, hq, d), normal(g, n, hkv, d), normal(g, n, hkv, d)
+        for causal in (True, False):
+            want = gpu_ctx.attention_varlen(q, k, v, offsets(lens), causal=causal)
+            here = q.clone()
+            assert gpu_ctx.attention_varlen(here, k, v, offsets(lens), causal=causal, out=here) is here
+            gpu_ctx.sync()
+            assert torch.equal(here, want)
+        klens = [3000, 45, 0, 129]
+        pq, cache = paged_case(g, hq, hkv, d, 16, klens, "bf16")
+        want = gpu_ctx.attention_paged(pq, cache, ints(klens))
+        assert gpu_ctx.attention_paged(pq, cache, ints(klens), out=pq) is pq
+        gpu_ctx.sync()
+        assert torch.equal(pq, want)
+    q, k, v = normal(g, n, 4, 64), normal(g, n, 4, 64), normal(g, n, 4, 64)
+    buf = normal(g, 2 * n, 4, 64)
+    _, cache = paged_case(g, 4, 4, 64, 16, [20, 20], "bf16")
+    fused = normal(g, 2, 12, 64)
+    lens2 = ints([20, 20])
+    for call in (lambda: gpu_ctx.attention_varlen(q, k, v, offsets(lens), out=k),
+                 lambda: gpu_ctx.attention_varlen(q, k, v, offsets(lens), out=v),
+                 lambda: gpu_ctx.attention_varlen(buf[:n], k, v, offsets(lens), out=buf[5:n + 5]),
+                 lambda: gpu_ctx.attention_varlen(q, buf[:n], v, offsets(lens), out=buf[n - 1:2 * n - 1]),
+                 lambda: gpu_ctx.attention_paged(buf[1:3], cache, lens2, out=buf[0:2]),
+                 lambda: gpu_ctx.kv_append(cache, k[:2], v[:2], lens2, q=q[:2], q_out=k[:2]),
+                 lambda: gpu_ctx.kv_append(cache, k[:2], v[:2], lens2, k_out=v[:2]),
+                 lambda: gpu_ctx.kv_append(cache, k[:2], v[:2], lens2, q=q[:2], q_out=buf[:2], k_out=buf[1:3]),
+                 lambda: gpu_ctx.kv_append(cache, k[:2], v[:2], lens2, q=q[:2], k_out=q[:2]),
+                 lambda: gpu_ctx.kv_append(cache, k[:2], v[:2], lens2, k_out=k[1:3]),
+                 lambda: gpu_ctx.kv_append(cache, fused[:, 4:8], fused[:, 8:], lens2, q=fused[:, :4],
+                                           q_out=fused.view(-1, 4, 64)[:2])):
+        with pytest.raises(HsError) as e:
+            call()
+        assert e.value.status == HS_ERR_INVALID
+    gpu_ctx.sync()
+    gpu_ctx.attention_varlen(buf[:n], k, v, offsets(lens), out=buf[n:])  # side by side in one buffer
+    gpu_ctx.kv_append(cache, fused[:, 4:8], fused[:, 8:], lens2, q=fused[:, :4], q_out=buf[:2], k_out=buf[2:4])
+    gpu_ctx.sync()
