@@ -32,25 +32,35 @@
 // the row sum (of the unrounded P, in packed adds: summing the rounded P costs
 // 3 % of the speed at 128 and 3 % at 64) and accumulators are f32.
 //
-// What bounds it (8,192 tokens, 32/8 x 128, not causal, one burst at 1,965 MHz:
-// 827 us, 1,329 TFLOP/s): per pair of 128 x 64 tiles about 1,850 cycles, of
-// which the tensor core's share is 1,260 (64-column score products run at two
-// thirds of its rate) and the MUFU's 900.  A softmax warp spends most of them
-// in the exponentials (both warpgroups at the same time, so at half the MUFU's
-// rate each), the rest in the maximum, in waits for scores and in the hand-over.
-// Under load the 1,000 W cap takes the clock to 1,550 MHz: 1,189 TFLOP/s for a
-// causal prompt of 16,384.  Head_dim 64 is bound by the exponentials as
-// attn_fwd_sm100 is: 837 TFLOP/s for 16,384 tokens, 16 x 64, not causal.  An
-// item's start and end cost about 6,000 cycles, three 96-key tiles' worth, and
-// the GPU hands out about 28 pending blocks a microsecond, which bounds
-// thousands of items that are shorter than 5 us each.  (Dealing half to seven
-// eighths of the items out by block index instead: 9 % faster there, up to
-// 7 % slower on ragged prompts.)
-// Steps kept, on these two in TFLOP/s: 1,215 / 790 -> tested waits 1,240 / 798
-// -> the next K/V tile awaited before P 1,278 / 825 -> P stored 16 columns at
-// a time 1,312 / 830 -> the FMA pipe's share last of each 16 pairs, masked
-// weights exactly zero 1,329 / 837 -> exponents of score differences, right for any
-// finite score, 1,290 / 834.  Built and not kept, against the 1,215 / 790:
+// What bounds it (8,192 tokens, 32/8 x 128, not causal, one burst at 1,965
+// MHz: 852 to 874 us on two GPUs, 1,258 to 1,290 TFLOP/s): per pair of 128 x
+// 64 tiles 1,910 cycles and more, of which the tensor core's share is 1,260
+// (64-column score products run at two thirds of its rate) and the
+// exponentials' on the MUFU 900.  No pipe is full (tensor 67 %, XU 58 %,
+// issue 53 % of the active cycles): a softmax warp spends most of them in
+// the exponentials (both warpgroups at the same time, so at half the MUFU's
+// rate each), the rest in the maximum, in waits for scores and in the
+// hand-over.  Under load the 1,000 W cap takes the clock to 1,510 MHz: 1,139
+// TFLOP/s for a causal prompt of 16,384.  Head_dim 64: 817 to 834 TFLOP/s
+// for 16,384 tokens, 16 x 64, not causal; on 8,192 causal tokens XU 55 %,
+// issue 58 %, tensor 37 % of the active cycles, and 20 % of the time SMs
+// wait for the last items.  12 images of 261 to 1,374 tokens: XU 43 %, issue
+// 50 %, SMs active for 80 % of the time.  Keys are not split: few queries
+// onto a long history load few SMs (16 onto 100,000 keys, 32/8 x 128: 8
+// CTAs, 934 us; the keys' bytes take 63).  Every CTA looks the offsets
+// through once for the longest run and then class by class, 32 sequences at
+// a time, which grows with the sequences.  An item's start and end cost
+// about 6,000 cycles, three 96-key tiles' worth, and the GPU hands out about
+// 28 pending blocks a microsecond, which bounds thousands of items that are
+// shorter than 5 us each.  (Dealing half to seven eighths of the items out
+// by block index instead: 9 % faster there, up to 7 % slower on ragged
+// prompts.)
+// Steps kept, on these two in TFLOP/s: 1,215 / 790 -> tested waits 1,240 /
+// 798 -> the next K/V tile awaited before P 1,278 / 825 -> P stored 16
+// columns at a time 1,312 / 830 -> the FMA pipe's share last of each 16
+// pairs, masked weights exactly zero 1,329 / 837 -> exponents of score
+// differences, right for any finite score, 1,290 / 834 where the step before
+// reached 1,333 / 850.  Built and not kept, against the 1,215 / 790:
 //   head_dim 128 with 128-key tiles and one score buffer (1,079; with one MMA
 //     warp for both warpgroups 1,170, without splitting P's hand-over 1,251 in
 //     a burst, 1,052 against 1,141 at the power cap)
@@ -381,7 +391,10 @@ __device__ void softmax_role(const Args& a, Ctrl<D>* ctl, uint32_t tmem, int war
                                                 kSiteODone, a.timeout_ns)
                                     : warp_wait(&ctl->pv_prev[wg], (base_bits >> 3) & 1, abort_flag, a.status,
                                                 kSiteODone, a.timeout_ns);
-        if (!ok) return;
+        if (!ok) {
+          tmem_wait_st();  // P's stores land before TMEM is freed
+          return;
+        }
         tc_fence_after();
         const float factor = need ? ex2_approx((m_old - m_run) * c) : 1.f;
         l *= factor;
@@ -860,10 +873,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 8) {
     regs_inc<kSoftmaxRegs>();
     softmax_role<E, D>(a, ctl, tmem, warp, lane);
-    // A role that gave up in the middle of a tile may have stores to TMEM in
-    // flight; they land before it is freed.
-    __syncwarp();
-    tmem_wait_st();
   } else {
     regs_dec<kControlRegs>();
     if (warp == kProducerWarp)
