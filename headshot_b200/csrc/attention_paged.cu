@@ -3,9 +3,12 @@
 //
 // For the g query heads that share a key head (Hq / Hkv, in tiles of 16):
 //   out_h = sum_j 2^(s_hj c - m_h) v_j / sum_j 2^(s_hj c - m_h),  s_hj = q_h.k_j
-// over the sequence's cached keys, c = scale log2 e.  Every K and V row is
-// read once (4 Hkv D bytes per key) for 4 Hq D flops per key, so HBM bounds
-// it; a single short sequence is bound by latency.
+// over the sequence's cached keys, c = scale log2 e.  A head tile reads every K
+// and V row once (4 D bytes per key and key head) for 4 D flops per key and
+// query head, so HBM bounds it; a single short sequence is bound by latency.
+// Above 16 query heads per key head each further 16 read the cache again: 64
+// sequences of 20,000 keys on one key head of 128, 16, 32 and 48 heads 112, 207
+// and 294 us, and DRAM carries the cache three times for 48.
 //
 // Work is cut in tiles of 64 or 128 keys of one (sequence, key head, head tile)
 // item, numbered through all items (an item has kItemCost numbers more than
@@ -34,9 +37,10 @@
 // rounded away, cost 5 % at head_dim 64.)  Keys past the length are never read
 // (the ring is zero-filled there).
 //
-// Measured: 128 sequences of 1 to 16,001 keys, 32/8 x 128: 166 us, 6.5 TB/s;
-// 274,800 keys, 16 x 64: 170 us, 6.6 TB/s (a plain copy reaches 6.55).  One
-// sequence of 8,191 keys, 32/8 x 128: 15.6 us for 5.1 us of reading: launch 1.1,
+// Measured in a graph of such calls: 128 sequences of 1 to 16,001 keys, 32/8 x
+// 128: 165 us, 6.6 TB/s; 274,800 keys, 16 x 64: 172 us, 6.6 TB/s (a plain copy
+// reaches 6.55).  Call by call, each on other caches: 184 and 192 us.  One
+// sequence of 8,191 keys, 32/8 x 128: 15.9 us for 5.1 us of reading: launch 1.1,
 // range 1.2, keys and values 8.3, join of the warps 0.9, partials written and
 // counted 1.0, 26 of them joined 3.2.
 #include <cuda_bf16.h>
@@ -59,9 +63,9 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: weights stay below 2^8
 
 // 8 KB of K and V per warp and tile either way.  Head_dim 128: three stages and
 // two CTAs per SM (255 registers; three CTAs of two stages spill, 1.9 times
-// slower).  Head_dim 64 (200 x 1,374 keys, 16 x 64): 170 us like this, 173 us
-// with three stages and two CTAs, 182 us with 16 keys per warp, four stages
-// and three CTAs.
+// slower).  Head_dim 64 (200 x 1,374 keys, 16 x 64): 170 us like this (168
+// registers, 44 bytes of spills), 173 us with three stages and two CTAs, 182 us
+// with 16 keys per warp, four stages and three CTAs.
 template <int D>
 struct Shape {
   static constexpr int kWarpKeys = D == 128 ? 16 : 32;
